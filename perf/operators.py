@@ -247,11 +247,11 @@ def prepare(case, seed):
         if own:
             # the step's plan and workspace: the scheduler makes them once, every layer's launch uses them
             from kvcache_amd import ops
-            work_list, units, records = ops.chunk_plan(s["q_lens"], s["kv_lens"], case["hq"], case["hkv"], case["d"],
-                                                       case["block"], kv_dtype=_kv_dtype(case),
-                                                       window=case["window"], tab_off=s["off"])
+            work_list, units, tiles, records = ops.chunk_plan(s["q_lens"], s["kv_lens"], case["hq"], case["hkv"],
+                                                              case["d"], case["block"], kv_dtype=_kv_dtype(case),
+                                                              window=case["window"], tab_off=s["off"])
             s["plan"] = torch.from_numpy(np.ascontiguousarray(work_list)).to(DEV)
-            s["units"], s["records"] = units, records
+            s["units"], s["tiles"], s["records"] = units, tiles, records
             size = ops.chunk_workspace_size(case["hq"], case["hkv"], case["d"], records)
             s["ws"] = torch.zeros(max(size, 256), dtype=torch.uint8, device=DEV)
     return _address(s)
@@ -316,8 +316,8 @@ def _own_attn(c, s):
     from kvcache_amd import ops
     p = s["p"]
     ops.paged_chunk_attn(p["q"], p["out"], p["k_pool"], p["v_pool"], p.get("scales"), p["table"], len(s["table"]),
-                         p["plan"], s["units"], s["records"], len(s["q"]), c["hq"], c["hkv"], c["d"], c["block"],
-                         s["scale"], kv_dtype=_kv_dtype(c), softcap=c["cap"], window=c["window"],
+                         p["plan"], s["units"], s["tiles"], s["records"], len(s["q"]), c["hq"], c["hkv"], c["d"],
+                         c["block"], s["scale"], kv_dtype=_kv_dtype(c), softcap=c["cap"], window=c["window"],
                          workspace=(p["ws"], s["ws"].numel()), stream=_stream())
     return s["out"]
 
