@@ -49,7 +49,8 @@ enum kvc_status {
     KVC_ERR_WORKSPACE = 5,   /* caller workspace smaller than required */
     KVC_ERR_STATE = 6        /* call not valid in the object's current state */
 };
-enum kvc_dtype { KVC_F32 = 0, KVC_F16 = 1 };
+/* KVC_I8, KVC_E4M3: cached rows held as 8-bit codes and scales ("8-bit paged caches" below) */
+enum kvc_dtype { KVC_F32 = 0, KVC_F16 = 1, KVC_I8 = 2, KVC_E4M3 = 3 };
 /* How an engine step launches decode: host-planned work list (kvc_decode_plan +
  * kvc_batched_paged_decode_planned) or device lengths (kvc_batched_paged_decode_split). */
 enum kvc_decode_path { KVC_DECODE_PLANNED = 0, KVC_DECODE_DEVICE_LENGTHS = 1 };
@@ -364,6 +365,66 @@ size_t kvc_paged_causal_attn_dev_workspace_size(int Nq, int Hq, int Hkv, int D, 
 int kvc_paged_causal_attn_dev_noalloc(const void* q, void* out, const void* k_pool, const void* v_pool,
                                       const int* block_table, const int* dev_q_pos_base, int Nq, int Hq, int Hkv,
                                       int D, int BLOCK, float scale, int dtype, kvc_stream_t stream);
+
+/* ---- 8-bit paged caches ------------------------------------------------
+ * No counterpart in the reference, whose caches hold the compute type.  A row x of one
+ * token and KV head (D values) is held as 8-bit codes c and a scale s, x ~ c s:
+ *   KVC_I8:   s = max|x| / 127, c = round(x / s)
+ *   KVC_E4M3: s = max|x| / 448, c = e4m3(x / s)          (both round half to even).
+ * A row of magnitudes below 2^-100 is held as zeros; one that holds an Inf or NaN gets s = NaN
+ * and codes 0 (it reads back as NaN).  Pools [num_blocks, Hkv, BLOCK, D] of codes (int8 or e4m3
+ * bytes); kv_scales [num_blocks, Hkv, BLOCK, 2] fp32, {of K, of V}, one array for both pools.
+ * head_dim 32, 64, 128 or 256; pools, rows and weights 16-byte aligned, scales 8-byte.
+ * slots[r] = phys * BLOCK + pos % BLOCK of row r (negative: the row is not written / read; its
+ * place is left as it was).  The slots >= 0 of one writing call must differ (a row's codes and
+ * scale are stored by several lanes: of two rows with one slot, parts of both may stay).
+ *
+ * kvc_qk_norm_rope_write: the rows q|k|v of a projection, qkv [M, (Hq + 2 Hkv) * D] fp16, row r
+ *   at r * row_stride elements (a multiple of 8; 0: packed).  Every head of q and k:
+ *   y = x / sqrt(mean(x^2) + eps) * w (q_norm / k_norm [D] fp16; NULL: no norm), then the
+ *   rotate-half rotary embedding at pos[r] (pairs (t, t + D/2), frequencies theta^(-2t/D); the
+ *   angles are exact to fp32 at any position).  q [M, Hq, D] fp16 gets every row; k and v go into
+ *   the pools of kv_dtype (KVC_F16: kv_scales NULL; KVC_I8, KVC_E4M3: quantised from fp32).
+ *   q must not overlap qkv.
+ * kvc_write_kv_q8: k, v [rows, Hkv, D] of dtype (KVC_F16, KVC_F32) into 8-bit pools.
+ * kvc_read_kv: rows of the pools (KVC_F16, KVC_I8, KVC_E4M3) as k, v [rows, Hkv, D] of dtype. */
+int kvc_qk_norm_rope_write(void* q, void* k_pool, void* v_pool, float* kv_scales, const void* qkv, long long row_stride,
+                           const int* pos, const int* slots, const void* q_norm, const void* k_norm, float eps,
+                           float theta, int M, int Hq, int Hkv, int D, int BLOCK, int kv_dtype, kvc_stream_t stream);
+int kvc_write_kv_q8(const void* k, const void* v, void* k_pool, void* v_pool, float* kv_scales, const int* slot_map,
+                    int rows, int Hkv, int D, int BLOCK, int dtype, int kv_dtype, kvc_stream_t stream);
+int kvc_read_kv(void* k, void* v, const void* k_pool, const void* v_pool, const float* kv_scales, const int* slot_map,
+                int rows, int Hkv, int D, int BLOCK, int dtype, int kv_dtype, kvc_stream_t stream);
+
+/* Attention of a ragged batch of chunks over a paged cache (KVC_F16, KVC_I8 or KVC_E4M3):
+ * sequence s brings q_lens[s] >= 0 new tokens (1: a decode step), whose K and V are already in
+ * the cache, and then holds kv_lens[s] >= q_lens[s] tokens.  Token i of it sits at position
+ * p = kv_lens[s] - q_lens[s] + i and attends to keys max(0, p - window + 1) .. p (window 0: from
+ * 0); scores are scale * q.k, with softcap > 0 softcap * tanh(score / softcap).  q and out are
+ * [rows, Hq, D] fp16, the sequences' tokens one after the other; statistics are fp32.  A row
+ * whose scores are all -Inf gets zeros; NaN and Inf in K or V reach the rows that see their key.
+ *
+ * kvc_chunk_plan (host, once per step): cuts the batch into units and writes them into `work`
+ *   (host memory of capacity * 16 ints; NULL: only counts).  capacity and *n_units are in
+ *   entries of 16 ints, the list's header (entry 0) included; *n_tiles says how many units are
+ *   tiles of many rows; *n_records is the partial rows of split key ranges.  host_tab_off
+ *   (N + 1, NULL: tables packed in sequence order) locates each sequence's table in table_all.
+ *   The caller copies the list to the device.
+ * kvc_paged_chunk_attn: runs it (same shape, kv_dtype and window; tuning knobs play no part).
+ *   Every table read is bounded by table_len, every row by rows.  n_units, n_tiles and n_records
+ *   may exceed the list's own counts (a captured graph replays lists of any smaller size that
+ *   are copied to the same address; n_tiles > 0 then admits lists with tiles, and with
+ *   n_tiles 0 a list that holds tiles leaves their rows unwritten).  workspace:
+ *   kvc_chunk_workspace_size bytes, 16-byte aligned, any contents; NULL: library-owned (not
+ *   under stream capture); launches that may overlap need workspaces of their own. */
+int kvc_chunk_plan(const int* host_q_lens, const int* host_kv_lens, const int* host_tab_off, int N, int Hq, int Hkv,
+                   int D, int BLOCK, int kv_dtype, int window, int* work, int capacity, int* n_units, int* n_tiles,
+                   int* n_records);
+size_t kvc_chunk_workspace_size(int Hq, int Hkv, int D, int n_records);
+int kvc_paged_chunk_attn(const void* q, void* out, const void* k_pool, const void* v_pool, const float* kv_scales,
+                         const int* table_all, int table_len, const int* work, int n_units, int n_tiles, int n_records,
+                         int rows, int Hq, int Hkv, int D, int BLOCK, float scale, float softcap, int window,
+                         int kv_dtype, void* workspace, size_t workspace_bytes, kvc_stream_t stream);
 
 /* ---- decoder-step operations around the attention path (a Qwen2-shaped layer) ----
  * fp16 activations and weights, fp32 arithmetic; row widths multiples of 8.

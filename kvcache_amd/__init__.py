@@ -10,6 +10,6 @@ Layers:
   kvcache_amd.engine     Python handles over the C++ Engine / run_static
   kvcache_amd.workloads  reference and BASELINE workload generators
 """
-from ._native import KVC_F16, KVC_F32, KvcError, LIB_PATH, lib  # noqa: F401
+from ._native import KVC_E4M3, KVC_F16, KVC_F32, KVC_I8, KvcError, LIB_PATH, lib  # noqa: F401
 
 __version__ = "0.1.0"

@@ -21,6 +21,8 @@ KVC_ERR_WORKSPACE = 5
 KVC_ERR_STATE = 6
 KVC_F32 = 0
 KVC_F16 = 1
+KVC_I8 = 2
+KVC_E4M3 = 3
 KVC_DECODE_PLANNED = 0
 KVC_DECODE_DEVICE_LENGTHS = 1
 
@@ -144,6 +146,14 @@ _SIGS = {
     "kvc_paged_causal_attn_dev": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, f32, i32, vp, sz, vp]),
     "kvc_paged_causal_attn_dev_workspace_size": (sz, [i32, i32, i32, i32, i32, i32]),
     "kvc_paged_causal_attn_dev_noalloc": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, f32, i32, vp]),
+    "kvc_qk_norm_rope_write": (
+        i32, [vp, vp, vp, vp, vp, C.c_longlong, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, i32, i32, vp]),
+    "kvc_write_kv_q8": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
+    "kvc_read_kv": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
+    "kvc_chunk_plan": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, i32, ip, ip, ip]),
+    "kvc_chunk_workspace_size": (sz, [i32, i32, i32, i32]),
+    "kvc_paged_chunk_attn": (
+        i32, [vp] * 6 + [i32, vp] + [i32] * 8 + [f32, f32, i32, i32, vp, sz, vp]),
     "kvc_embed_gather": (i32, [vp, vp, vp, i32, i32, i32, vp]),
     "kvc_rmsnorm": (i32, [vp, vp, vp, i32, i32, f32, vp]),
     "kvc_add_bias": (i32, [vp, vp, i32, i32, vp]),

@@ -261,6 +261,8 @@ std::vector<int*> g_err_words;
 
 }  // namespace
 
+int library_workspace(size_t bytes, hipStream_t st, void** out) { return default_workspace(bytes, st, out); }
+
 int* device_error_word(hipStream_t st, bool may_alloc) {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return nullptr;

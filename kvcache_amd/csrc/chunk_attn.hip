@@ -1,0 +1,223 @@
+// chunk_attn.hip -- attention of a ragged batch of chunks over a paged cache: the host plan and
+// the launches (kernels in chunk_attn.hpp).
+#include "chunk_attn.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+#include <vector>
+
+namespace kvc {
+namespace {
+
+constexpr size_t kPartAlign = 256;
+size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+size_t acc_bytes(int Hkv, int D, int n_records) { return up((size_t)Hkv * n_records * D * sizeof(float), kPartAlign); }
+size_t ml_bytes(int Hkv, int n_records) { return up((size_t)Hkv * n_records * 2 * sizeof(float), kPartAlign); }
+
+int check_shape(int Hq, int Hkv, int D, int BLOCK, int kv_dtype, int window) {
+    if (kv_dtype == KVC_F32) return set_error(KVC_ERR_UNSUPPORTED, "the cache must be KVC_F16, KVC_I8 or KVC_E4M3");
+    if (kv_dtype != KVC_F16 && kv_dtype != KVC_I8 && kv_dtype != KVC_E4M3)
+        return set_error(KVC_ERR_ARG, "kv_dtype must be KVC_F16, KVC_I8 or KVC_E4M3");
+    if (Hq <= 0 || Hkv <= 0 || Hq % Hkv) return set_error(KVC_ERR_ARG, "Hq must be a positive multiple of Hkv");
+    if (D != 32 && D != 64 && D != 128 && D != 256)
+        return set_error(KVC_ERR_UNSUPPORTED, "head_dim must be 32, 64, 128 or 256");
+    if (BLOCK <= 0 || window < 0) return set_error(KVC_ERR_ARG, "BLOCK must be > 0 and window >= 0");
+    return KVC_OK;
+}
+
+// One tile of rows before its key range is cut.
+struct Tile {
+    int kind, row0, ntok, pos0, h0, hn, j0, j1, tab;
+};
+
+struct PlanUnit {
+    int f[kChunkInts];
+    long long cost;
+};
+
+// The batch as units.  Rows come in tiles of at most kRowsPerUnit (token, head) pairs.
+constexpr int kRowsPerUnit = 16;
+constexpr int kChunkKeys = 1024;
+void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N, int Hq, int Hkv, int BLOCK, int window,
+                std::vector<PlanUnit>& units, long long& records) {
+    const int group = Hq / Hkv;
+    std::vector<Tile> tiles;
+    long long row = 0, tab = 0;
+    for (int s = 0; s < N; ++s) {
+        const int nq = q_lens[s], nk = kv_lens[s];
+        if (tab_off) tab = tab_off[s];
+        const int hstep = std::min(group, kRowsPerUnit), tstep = std::max(1, kRowsPerUnit / group);
+        for (int i = 0; i < nq; i += tstep)
+            for (int h = 0; h < group; h += hstep) {
+                Tile t{kKindRows, (int)row + i, std::min(tstep, nq - i), nk - nq + i, h, std::min(hstep, group - h), 0, 0,
+                       (int)tab};
+                t.j1 = t.pos0 + t.ntok;
+                t.j0 = window > 0 ? std::max(0, t.pos0 - window + 1) / 64 * 64 : 0;
+                tiles.push_back(t);
+            }
+        row += nq;
+        if (!tab_off) tab += ((long long)nk + BLOCK - 1) / BLOCK;
+    }
+    records = 0;
+    for (const Tile& t : tiles) {
+        const int len = t.j1 - t.j0;
+        int nc = std::max(1, (len + kChunkKeys - 1) / kChunkKeys);
+        const int step = ((len + nc - 1) / nc + 63) / 64 * 64;
+        nc = (len + step - 1) / step;
+        const int rows = t.ntok * t.hn;
+        for (int c = 0; c < nc; ++c) {
+            PlanUnit u{};
+            u.f[kFKind] = t.kind;
+            u.f[kFRow] = t.row0;
+            u.f[kFTok] = t.ntok;
+            u.f[kFPos] = t.pos0;
+            u.f[kFHead] = t.h0;
+            u.f[kFHeads] = t.hn;
+            u.f[kFJ0] = t.j0 + c * step;
+            u.f[kFJ1] = std::min(t.j1, t.j0 + (c + 1) * step);
+            u.f[kFChunk] = c;
+            u.f[kFChunks] = nc;
+            u.f[kFRec] = nc > 1 ? (int)std::min<long long>(records, INT_MAX) : 0;
+            u.f[kFTab] = t.tab;
+            u.cost = (long long)(u.f[kFJ1] - u.f[kFJ0]) * rows;
+            units.push_back(u);
+        }
+        if (nc > 1) records += (long long)nc * rows;
+    }
+    std::stable_sort(units.begin(), units.end(), [](const PlanUnit& a, const PlanUnit& b) { return a.cost > b.cost; });
+}
+
+template <typename F>
+int guard_chunk(F&& f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc&) {
+        return set_error(KVC_ERR_NOMEM, "out of host memory");
+    } catch (...) {
+        return set_error(KVC_ERR_STATE, "unexpected exception");
+    }
+}
+
+template <int D, int CT>
+int launch_chunks_d(const ChunkParams& p, hipStream_t st) {
+    const dim3 grid((unsigned)((size_t)(p.n_units - 1) * p.Hkv));
+    hipLaunchKernelGGL((chunk_rows_kernel<D, CT>), grid, dim3(256), 0, st, p);
+    int rc = hip_check(hipGetLastError(), "chunk attention launch");
+    if (rc || p.n_records == 0) return rc;
+    hipLaunchKernelGGL((merge_chunks_kernel<D>), grid, dim3(256), 0, st, p);
+    return hip_check(hipGetLastError(), "chunk attention merge launch");
+}
+
+template <int D>
+int launch_chunks(const ChunkParams& p, int kv_dtype, hipStream_t st) {
+    if (kv_dtype == KVC_F16) return launch_chunks_d<D, kCacheF16>(p, st);
+    if (kv_dtype == KVC_I8) return launch_chunks_d<D, kCacheI8>(p, st);
+    return launch_chunks_d<D, kCacheE4M3>(p, st);
+}
+
+}  // namespace
+}  // namespace kvc
+
+using namespace kvc;
+
+extern "C" {
+
+int kvc_chunk_plan(const int* host_q_lens, const int* host_kv_lens, const int* host_tab_off, int N, int Hq, int Hkv,
+                   int D, int BLOCK, int kv_dtype, int window, int* work, int capacity, int* n_units, int* n_tiles,
+                   int* n_records) {
+    return guard_chunk([&]() -> int {
+        int rc = check_shape(Hq, Hkv, D, BLOCK, kv_dtype, window);
+        if (rc) return rc;
+        if (N < 0 || !n_units || !n_tiles || !n_records) return set_error(KVC_ERR_ARG, "N must be >= 0 and the counts not null");
+        if (N > 0 && (!host_q_lens || !host_kv_lens)) return set_error(KVC_ERR_ARG, "null lengths");
+        long long rows = 0, blocks = 0;
+        for (int s = 0; s < N; ++s) {
+            if (host_q_lens[s] < 0 || host_kv_lens[s] < host_q_lens[s])
+                return set_error(KVC_ERR_ARG, "sequence " + std::to_string(s) + ": 0 <= q_lens <= kv_lens is needed");
+            if (host_tab_off && host_tab_off[s] < 0) return set_error(KVC_ERR_ARG, "negative table offset");
+            rows += host_q_lens[s];
+            blocks += ((long long)host_kv_lens[s] + BLOCK - 1) / BLOCK;
+        }
+        if (rows > INT_MAX || blocks > INT_MAX) return set_error(KVC_ERR_UNSUPPORTED, "at most 2^31 - 1 rows and table entries");
+        std::vector<PlanUnit> units;
+        long long records = 0;
+        plan_units(host_q_lens, host_kv_lens, host_tab_off, N, Hq, Hkv, BLOCK, window, units, records);
+        if (records > INT_MAX || ((long long)units.size() + 1) * Hkv > INT_MAX)
+            return set_error(KVC_ERR_UNSUPPORTED, "the batch needs more than 2^31 - 1 units or partial rows");
+        *n_units = (int)units.size() + 1;
+        *n_tiles = (int)std::count_if(units.begin(), units.end(), [](const PlanUnit& u) { return u.f[kFKind] == kKindTile; });
+        *n_records = (int)records;
+        if (!work) return KVC_OK;
+        if (capacity < *n_units)
+            return set_error(KVC_ERR_ARG, "work list too small: " + std::to_string(*n_units) + " entries of 16 ints are needed");
+        std::fill(work, work + kChunkInts, 0);
+        work[kHdrUnits] = *n_units;
+        work[kHdrTiles] = *n_tiles;
+        work[kHdrRecords] = *n_records;
+        for (size_t i = 0; i < units.size(); ++i) std::copy(units[i].f, units[i].f + kChunkInts, work + (i + 1) * kChunkInts);
+        return KVC_OK;
+    });
+}
+
+size_t kvc_chunk_workspace_size(int Hq, int Hkv, int D, int n_records) {
+    if (Hq <= 0 || Hkv <= 0 || D <= 0 || n_records <= 0) return 0;
+    return acc_bytes(Hkv, D, n_records) + ml_bytes(Hkv, n_records);
+}
+
+int kvc_paged_chunk_attn(const void* q, void* out, const void* k_pool, const void* v_pool, const float* kv_scales,
+                         const int* table_all, int table_len, const int* work, int n_units, int n_tiles, int n_records,
+                         int rows, int Hq, int Hkv, int D, int BLOCK, float scale, float softcap, int window,
+                         int kv_dtype, void* workspace, size_t workspace_bytes, kvc_stream_t stream) {
+    return guard_chunk([&]() -> int {
+        int rc = check_shape(Hq, Hkv, D, BLOCK, kv_dtype, window);
+        if (rc) return rc;
+        if (rows < 0 || n_units < 0 || n_tiles < 0 || n_records < 0)
+            return set_error(KVC_ERR_ARG, "rows and the plan's counts must be >= 0");
+        if (!std::isfinite(scale)) return set_error(KVC_ERR_ARG, "scale must be finite");
+        if (!(softcap >= 0.f) || !std::isfinite(softcap)) return set_error(KVC_ERR_ARG, "softcap must be >= 0 and finite");
+        if (rows == 0 || n_units <= 1) return KVC_OK;
+        if ((long long)n_units * Hkv > INT_MAX) return set_error(KVC_ERR_UNSUPPORTED, "at most 2^31 - 1 workgroups");
+        if (!q || !out || !k_pool || !v_pool || !table_all || table_len <= 0 || !work)
+            return set_error(KVC_ERR_ARG, "null q, out, pool, table or work list");
+        auto al = [](const void* x) { return ((uintptr_t)x & 15u) == 0; };
+        if (!al(q) || !al(out) || !al(k_pool) || !al(v_pool) || ((uintptr_t)work & 3u))
+            return set_error(KVC_ERR_ARG, "q, out and the pools must be 16-byte aligned");
+        if (kv_dtype != KVC_F16 && (!kv_scales || ((uintptr_t)kv_scales & 7u)))
+            return set_error(KVC_ERR_ARG, "an 8-bit cache needs its scales, 8-byte aligned");
+        ChunkParams p{};
+        const float log2e = 1.4426950408889634f;
+        p.work = work; p.n_units = n_units; p.n_records = n_records;
+        p.rows = rows; p.Hq = Hq; p.Hkv = Hkv; p.group = Hq / Hkv; p.block = BLOCK;
+        p.table_len = table_len; p.window = window;
+        p.scale_log2 = scale * log2e;
+        p.cap_log2 = softcap * log2e;
+        p.cap_in = softcap > 0.f ? 2.f * scale * log2e / softcap : 0.f;
+        p.q = static_cast<const _Float16*>(q);
+        p.out = static_cast<_Float16*>(out);
+        p.k = k_pool; p.v = v_pool; p.scales = kv_scales; p.table = table_all;
+        if (n_records > 0) {
+            const size_t need = kvc_chunk_workspace_size(Hq, Hkv, D, n_records);
+            if (!workspace) {
+                rc = library_workspace(need, (hipStream_t)stream, &workspace);
+                if (rc) return rc;
+            } else if (workspace_bytes < need) {
+                return set_error(KVC_ERR_WORKSPACE, "workspace too small: need " + std::to_string(need) + " bytes, got " +
+                                                        std::to_string(workspace_bytes));
+            } else if (!al(workspace)) {
+                return set_error(KVC_ERR_ARG, "workspace must be 16-byte aligned");
+            }
+            p.part_acc = static_cast<float*>(workspace);
+            p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + acc_bytes(Hkv, D, n_records));
+        }
+        const hipStream_t st = (hipStream_t)stream;
+        switch (D) {
+            case 32: return launch_chunks<32>(p, kv_dtype, st);
+            case 64: return launch_chunks<64>(p, kv_dtype, st);
+            case 128: return launch_chunks<128>(p, kv_dtype, st);
+            default: return launch_chunks<256>(p, kv_dtype, st);
+        }
+    });
+}
+
+}  // extern "C"

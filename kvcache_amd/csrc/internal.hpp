@@ -13,6 +13,10 @@ namespace kvc {
 // Checks a HIP return code; on failure records it and returns KVC_ERR_HIP.
 int hip_check(hipError_t e, const char* what);
 
+// The library's grow-only workspace of (current device, stream), for calls that bring none;
+// KVC_ERR_STATE while the stream is capturing (abi.hip).
+int library_workspace(size_t bytes, hipStream_t st, void** out);
+
 // ---------------------------------------------------------------------------
 // Decode launch description (host side).  One "unit" = (sequence s, KV head hk,
 // query-head subgroup sub, chunk c); each unit is one workgroup of `wpb` waves.

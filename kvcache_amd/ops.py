@@ -10,7 +10,7 @@ drivers call the CUDA launchers.
 """
 from __future__ import annotations
 
-from ._native import KVC_ERR_ARG, KVC_F16, KVC_F32, KvcError, check, lib
+from ._native import KVC_E4M3, KVC_ERR_ARG, KVC_F16, KVC_F32, KVC_I8, KvcError, check, lib
 from .device import DeviceBuffer
 
 __all__ = [
@@ -19,7 +19,8 @@ __all__ = [
     "qk_batched_paged_decode_attn", "write_kv_slots", "decode_workspace_size", "decode_auto_split",
     "decode_plan", "planned_workspace_size", "launch_batched_paged_planned", "launch_batched_paged_append_planned",
     "flash_decode_workspace_size", "qk_paged_causal_attn", "qkcuda_paged_causal_attn", "qkcuda_write_kv",
-    "qkcuda_rope", "check_device_errors", "stream_is_capturing", "KVC_F16", "KVC_F32",
+    "qkcuda_rope", "check_device_errors", "stream_is_capturing", "qk_norm_rope_write", "write_kv_q8", "read_kv",
+    "chunk_plan", "chunk_workspace_size", "paged_chunk_attn", "KVC_F16", "KVC_F32", "KVC_I8", "KVC_E4M3",
 ]
 
 
@@ -189,6 +190,69 @@ def qkcuda_write_kv(k, v, k_pool, v_pool, block_table_dev, dev_start_pos, L, Hkv
 def qkcuda_rope(x, L, n_heads, D, dev_pos_base, theta, *, stream=None):
     """qwen_kernels.h:42: qk_rope with pos_base in device memory."""
     check(lib().kvc_rope_dev(_p(x), _p(dev_pos_base), L, n_heads, D, theta, stream))
+
+
+# ---- 8-bit paged caches: norm + rotary + write, quantised write, read, attention of chunks --------
+def qk_norm_rope_write(q, k_pool, v_pool, kv_scales, qkv, pos, slots, M, Hq, Hkv, D, BLOCK, theta, *, row_stride=0,
+                       q_norm=None, k_norm=None, eps=1e-6, kv_dtype=KVC_I8, stream=None):
+    """q|k|v rows: RMSNorm of every q and k head, rotary at pos[r], q to its rows, k and v into
+    the paged cache (kvc_qk_norm_rope_write)."""
+    check(lib().kvc_qk_norm_rope_write(_p(q), _p(k_pool), _p(v_pool), _p(kv_scales), _p(qkv), row_stride, _p(pos),
+                                       _p(slots), _p(q_norm), _p(k_norm), eps, theta, M, Hq, Hkv, D, BLOCK, kv_dtype,
+                                       stream))
+
+
+def write_kv_q8(k, v, k_pool, v_pool, kv_scales, slot_map, rows, Hkv, D, BLOCK, *, dtype=KVC_F16, kv_dtype=KVC_I8,
+                stream=None):
+    """k, v [rows, Hkv, D] into 8-bit pools at their slots, one scale per row of a head."""
+    check(lib().kvc_write_kv_q8(_p(k), _p(v), _p(k_pool), _p(v_pool), _p(kv_scales), _p(slot_map), rows, Hkv, D, BLOCK,
+                                dtype, kv_dtype, stream))
+
+
+def read_kv(k, v, k_pool, v_pool, kv_scales, slot_map, rows, Hkv, D, BLOCK, *, dtype=KVC_F16, kv_dtype=KVC_I8,
+            stream=None):
+    """Rows of a paged cache (fp16 or 8-bit) as k, v [rows, Hkv, D]."""
+    check(lib().kvc_read_kv(_p(k), _p(v), _p(k_pool), _p(v_pool), _p(kv_scales), _p(slot_map), rows, Hkv, D, BLOCK,
+                            dtype, kv_dtype, stream))
+
+
+def chunk_plan(q_lens, kv_lens, Hq, Hkv, D, BLOCK, *, tab_off=None, kv_dtype=KVC_I8, window=0):
+    """Host-side plan of paged_chunk_attn (kvc_chunk_plan): returns (work [n_units, 16] int32,
+    n_units, n_tiles, n_records)."""
+    import ctypes as C
+
+    import numpy as np
+    q = np.ascontiguousarray(np.asarray(q_lens, dtype=np.int32))
+    t = np.ascontiguousarray(np.asarray(kv_lens, dtype=np.int32))
+    toff = None if tab_off is None else np.ascontiguousarray(np.asarray(tab_off, dtype=np.int32))
+    if q.shape != t.shape or q.ndim != 1 or (toff is not None and toff.shape != (len(q) + 1,)):
+        raise KvcError(KVC_ERR_ARG, "q_lens and kv_lens hold one length per sequence, tab_off one entry more")
+    tp = None if toff is None else toff.ctypes.data
+    nu, nt, nr = C.c_int(0), C.c_int(0), C.c_int(0)
+    L = lib()
+
+    def plan(work, cap):
+        check(L.kvc_chunk_plan(q.ctypes.data, t.ctypes.data, tp, len(q), Hq, Hkv, D, BLOCK, kv_dtype, window, work, cap,
+                               C.byref(nu), C.byref(nt), C.byref(nr)))
+
+    plan(None, 0)
+    work = np.zeros((nu.value, 16), dtype=np.int32)
+    plan(work.ctypes.data, nu.value)
+    return work, nu.value, nt.value, nr.value
+
+
+def chunk_workspace_size(Hq, Hkv, D, n_records) -> int:
+    return int(lib().kvc_chunk_workspace_size(Hq, Hkv, D, n_records))
+
+
+def paged_chunk_attn(q, out, k_pool, v_pool, kv_scales, table_all, table_len, work_dev, n_units, n_tiles, n_records,
+                     rows, Hq, Hkv, D, BLOCK, scale, *, kv_dtype=KVC_I8, softcap=0.0, window=0, workspace=None,
+                     stream=None):
+    """Attention of a ragged batch of chunks over a paged cache, on a plan of chunk_plan."""
+    ws, wsb = _ws(workspace)
+    check(lib().kvc_paged_chunk_attn(_p(q), _p(out), _p(k_pool), _p(v_pool), _p(kv_scales), _p(table_all),
+                                     int(table_len), _p(work_dev), n_units, n_tiles, n_records, rows, Hq, Hkv, D,
+                                     BLOCK, scale, softcap, window, kv_dtype, ws, wsb, stream))
 
 
 # ---- decoder-step operations (qwen_kernels.h:7-13,22-24) -----------------------------
