@@ -26,6 +26,10 @@ int check_shape(int Hq, int Hkv, int D, int BLOCK, int kv_dtype, int window) {
     return KVC_OK;
 }
 
+// The matrix-core kernels: head_dim 64 or 128, and blocks that hold whole 16-row subtiles,
+// found by a shift.
+bool matrix_path(int D, int BLOCK) { return (D == 64 || D == 128) && BLOCK >= 16 && (BLOCK & (BLOCK - 1)) == 0; }
+
 // One tile of rows before its key range is cut.
 struct Tile {
     int kind, row0, ntok, pos0, h0, hn, j0, j1, tab;
@@ -36,12 +40,12 @@ struct PlanUnit {
     long long cost;
 };
 
-// The batch as units.  Rows come in tiles of at most kRowsPerUnit (token, head) pairs.
-constexpr int kRowsPerUnit = 16;
+// The batch as units.
 constexpr int kChunkKeys = 1024;
-void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N, int Hq, int Hkv, int BLOCK, int window,
-                std::vector<PlanUnit>& units, long long& records) {
+void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N, int Hq, int Hkv, int D, int BLOCK,
+                int window, std::vector<PlanUnit>& units, long long& records) {
     const int group = Hq / Hkv;
+    const int kRowsPerUnit = matrix_path(D, BLOCK) ? 32 : 16;
     std::vector<Tile> tiles;
     long long row = 0, tab = 0;
     for (int s = 0; s < N; ++s) {
@@ -102,7 +106,14 @@ int guard_chunk(F&& f) {
 template <int D, int CT>
 int launch_chunks_d(const ChunkParams& p, hipStream_t st) {
     const dim3 grid((unsigned)((size_t)(p.n_units - 1) * p.Hkv));
-    hipLaunchKernelGGL((chunk_rows_kernel<D, CT>), grid, dim3(256), 0, st, p);
+    bool done = false;
+    if constexpr (D == 64 || D == 128) {
+        if (matrix_path(D, p.block)) {
+            hipLaunchKernelGGL((chunk_stream_kernel<D, CT>), grid, dim3(StreamShape<D, CT>::W * kWave), 0, st, p);
+            done = true;
+        }
+    }
+    if (!done) hipLaunchKernelGGL((chunk_rows_kernel<D, CT>), grid, dim3(256), 0, st, p);
     int rc = hip_check(hipGetLastError(), "chunk attention launch");
     if (rc || p.n_records == 0) return rc;
     hipLaunchKernelGGL((merge_chunks_kernel<D>), grid, dim3(256), 0, st, p);
@@ -142,7 +153,7 @@ int kvc_chunk_plan(const int* host_q_lens, const int* host_kv_lens, const int* h
         if (rows > INT_MAX || blocks > INT_MAX) return set_error(KVC_ERR_UNSUPPORTED, "at most 2^31 - 1 rows and table entries");
         std::vector<PlanUnit> units;
         long long records = 0;
-        plan_units(host_q_lens, host_kv_lens, host_tab_off, N, Hq, Hkv, BLOCK, window, units, records);
+        plan_units(host_q_lens, host_kv_lens, host_tab_off, N, Hq, Hkv, D, BLOCK, window, units, records);
         if (records > INT_MAX || ((long long)units.size() + 1) * Hkv > INT_MAX)
             return set_error(KVC_ERR_UNSUPPORTED, "the batch needs more than 2^31 - 1 units or partial rows");
         *n_units = (int)units.size() + 1;

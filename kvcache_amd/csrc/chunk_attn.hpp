@@ -168,6 +168,393 @@ __global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkParams p) {
     }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Few rows (at most 16 R of a KV head: decode steps, short chunks) on the matrix cores.
+//
+// A wave streams key tiles of its own, W waves of a workgroup taking tiles in turn; the next
+// tile's rows are on their way into registers while this one's are computed.
+//   S^T[key][row] = K Q^T with v_mfma_f32_16x16x32_f16: the result gives lane l the scores of
+//     row l % 16 for keys 4 (l / 16) + r of each 16-key subtile.  8-bit K is read from LDS 16
+//     codes at a time and turned into fp16 exactly; lane l's 16 codes are dims 64 j + 16 (l /
+//     16) .. + 15, two k steps of the product, and q lies in that order of dims.  The key's
+//     scale multiplies the score.
+//   softmax online in log2 units, fp32.
+//   O[row][dim] += P V: P is the lane's own scores' probabilities (keys 4 g + r of two
+//     subtiles, g = l / 16), V is read back transposed: 8-bit rows with ds_read_b64_tr_b8 (of
+//     16 lanes, lane i receives byte i % 8 of the 8 bytes that lanes 2 j + i / 8 address, j =
+//     0 .. 7: one dim of eight keys), fp16 rows with ds_read_b64_tr_b16.  The key's V scale
+//     goes onto its probability, in fp32 and before the rounding to fp16, in units of 2^(E - 15)
+//     with 2^E above every V scale met so far (O is kept in them): products of up to 2^15, so
+//     that fp16 has all its bits down to 2^-29 of the largest (in units of 2^E, V rows of sizes
+//     2^+-9 cost 2^-8 where a row's weight lay on small ones).  fp16 caches: probabilities are
+//     kept times 2^15 for the same reason.
+// LDS rows are 16-byte pieces permuted by the row, so that the sixteen rows one operand read
+// touches at the same piece lie on different banks.
+constexpr int kProbBits = 15;  // probabilities (times V scales) go up to 2^15
+
+template <int D, int CT>
+struct StreamShape {
+    static constexpr int CB = kCodeBytes<CT>;
+    static constexpr int ROW = D * CB;              // bytes of a cached row
+    static constexpr int KT = CB == 1 ? 64 : 32;    // keys per tile
+    static constexpr int SUB = KT / 16;             // 16-key subtiles
+    static constexpr int VL = 16 * ROW / 1024;      // 1 KiB wave loads per subtile
+    static constexpr int KD = D / 32;               // k steps over the head dimension
+    static constexpr int NT = D / 16;               // 16-dim output tiles
+    static constexpr int kTile = KT * ROW;          // bytes of a K (or V) tile
+    static constexpr int W = D == 64 ? 8 : 4;       // waves of a workgroup
+    // per wave: the K and V tiles, and the keys' factors
+    static constexpr int kWaveBytes = 2 * kTile + 2 * KT * 4;
+    static constexpr int kBytes = W * kWaveBytes;
+};
+
+__device__ __forceinline__ u32x2 ds_read_tr8(const char* p) {
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+        (__attribute__((address_space(3))) v2i*)(__attribute__((address_space(3))) char*)(const_cast<char*>(p))));
+}
+
+// fp16 caches: Inf and NaN in V.  A key that a row does not see has probability 0, and 0 x Inf
+// is NaN, so in the tiles that some row does not see whole the elements of V that are not finite
+// are staged as 0; a unit that met one adds them to the rows that see their key: acc += the
+// elements d0 .. d0 + 3 of V that are Inf or NaN, of the unit's keys that position pos sees.
+// (Those of tiles that were seen whole are in acc already and change nothing.)
+template <int D>
+__device__ __forceinline__ f32x4 add_seen_nonfinite(const ChunkParams& p, const ChunkUnit& u, f32x4 acc, int pos, int d0) {
+    const int bsh = __builtin_ctz((unsigned)p.block);
+    const int first = max(u.j0, p.window > 0 ? pos - p.window + 1 : 0), last = min(u.j1 - 1, pos);
+    for (int j = first; j <= last; ++j) {
+        const int id = p.table[min(u.tab + (j >> bsh), p.table_len - 1)];
+        const size_t row = (((size_t)(unsigned)(id * p.Hkv + u.hk)) << bsh) + (j & (p.block - 1));
+        const f16x4 v = *reinterpret_cast<const f16x4*>(static_cast<const _Float16*>(p.v) + row * D + d0);
+        const u16x4 bits = __builtin_bit_cast(u16x4, v);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (nonfinite(bits[r])) acc[r] += (float)v[r];
+    }
+    return acc;
+}
+
+template <int D, int CT, int R>
+__device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUnit& u, char* lds) {
+    using Sh = StreamShape<D, CT>;
+    constexpr int ROW = Sh::ROW, KT = Sh::KT, SUB = Sh::SUB, VL = Sh::VL, KD = Sh::KD, NT = Sh::NT, W = Sh::W;
+    constexpr bool Q8 = CT != kCacheF16;
+    const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6);
+    const int n16 = lane & 15, g4 = lane >> 4;
+    const int j0 = u.j0, j1 = u.j1;
+    const int ntiles = (j1 - j0 + KT - 1) / KT;
+    const int kmax = wave < ntiles ? (ntiles - wave + W - 1) / W : 0;
+    const int bsh = __builtin_ctz((unsigned)p.block), bmask = p.block - 1;
+    const char* kb = static_cast<const char*>(p.k);
+    const char* vb = static_cast<const char*>(p.v);
+
+    // block ids of this wave's subtiles, one per lane, 64 at a time
+    auto first_tok = [&](int s) { return j0 + (wave + W * (s / SUB)) * KT + 16 * (s % SUB); };
+    int ids = 0;
+    auto load_ids = [&](int s) {
+        const int t = min(first_tok(s + lane), j1 - 1);
+        ids = p.table[min(u.tab + (t >> bsh), p.table_len - 1)];
+    };
+    struct Tile {
+        u32x4 k[SUB][VL], v[SUB][VL];
+        f32x2 sc;
+    };
+    auto issue = [&](int k, Tile& T) {
+        const int t0 = j0 + (wave + W * k) * KT;
+        if constexpr (Q8) {  // lane = key; the block of a key past the range is its last one
+            const int id = __builtin_amdgcn_ds_bpermute(((SUB * k + g4) & (kWave - 1)) << 2, ids);
+            const size_t row = (((size_t)(unsigned)(id * p.Hkv + u.hk)) << bsh) + ((t0 + lane) & bmask);
+            T.sc = *reinterpret_cast<const f32x2*>(p.scales + row * 2);
+        }
+#pragma unroll
+        for (int h = 0; h < SUB; ++h) {
+            const int t = t0 + 16 * h;
+            const int id = __builtin_amdgcn_readlane(ids, (SUB * k + h) & (kWave - 1));
+            int rows = max(j1 - t, 0);
+            asm("" : "+s"(rows));
+            const int bytes = min(rows, 16) * ROW;
+            const size_t off = ((((size_t)(unsigned)(id * p.Hkv + u.hk)) << bsh) + (t & bmask)) * ROW;
+            const __amdgpu_buffer_rsrc_t kr = tile_rsrc(kb + off, bytes), vr = tile_rsrc(vb + off, bytes);
+#pragma unroll
+            for (int i = 0; i < VL; ++i) T.k[h][i] = buffer_load16(kr, i * 1024 + lane * 16);
+#pragma unroll
+            for (int i = 0; i < VL; ++i) T.v[h][i] = buffer_load16(vr, i * 1024 + lane * 16);
+        }
+    };
+
+    char* kt = lds + wave * Sh::kWaveBytes;
+    char* vt = kt + Sh::kTile;
+    float* s_k = reinterpret_cast<float*>(vt + Sh::kTile);  // factor of a key's score
+    float* s_v = s_k + KT;                                   // and of its probability
+    // 16-byte piece of a row in LDS (fp16 V: 32-byte segment)
+    auto piece = [](int r, int c) {
+        if constexpr (Q8) return c ^ (D == 64 ? (r >> 2) & 3 : (r >> 1) & 7);
+        else return c ^ (r & 7);
+    };
+    auto vseg = [](int r, int seg) { return seg ^ (D == 64 ? (r >> 1) & 3 : r & 7); };
+
+    Tile A, B;
+    if (kmax > 0) {
+        load_ids(0);
+        issue(0, A);
+    }
+    // q as the B operand: lane l holds row l % 16; 8-bit: dims 64 j + 16 g + 8 e .. + 7 in step 2 j + e
+    f16x8v qb[R][KD];
+    int pos[R];
+#pragma unroll
+    for (int a = 0; a < R; ++a) {
+        const int r = min(16 * a + n16, u.rows - 1);
+        pos[a] = u.pos0 + r / u.hn;
+        const _Float16* q = p.q + chunk_row(p, u, r, D);
+#pragma unroll
+        for (int d = 0; d < KD; ++d)
+            qb[a][d] = *reinterpret_cast<const f16x8v*>(q + (Q8 ? 64 * (d >> 1) + 16 * g4 + 8 * (d & 1) : 32 * d + 8 * g4));
+    }
+    const bool cap = p.cap_log2 > 0.f;
+    const float to_log2 = cap ? p.cap_in : p.scale_log2;
+    float m[R], l[R];
+    f32x4 O[R][NT];
+    int E = -126;
+#pragma unroll
+    for (int a = 0; a < R; ++a) {
+        m[a] = -FLT_MAX;
+        l[a] = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) O[a][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    bool bad = false;  // this wave cleared elements of V in tiles that some row does not see whole
+    // FULL: every key of the tile is seen by every row
+    auto consume = [&](int k, Tile& T, auto full_tag) {
+        constexpr bool FULL = decltype(full_tag)::value;
+        const int t0 = j0 + (wave + W * k) * KT;
+        if constexpr (!Q8 && !FULL) {
+            bool b = false;
+#pragma unroll
+            for (int h = 0; h < SUB; ++h) b |= any_nonfinite(T.v[h]);
+            if (b) {
+                bad = true;
+#pragma unroll
+                for (int h = 0; h < SUB; ++h) clear_nonfinite(T.v[h]);
+            }
+        }
+        float efac = 1.f;
+        if constexpr (Q8) {
+            float ks = T.sc[0], vs = T.sc[1];
+            if (!FULL && t0 + lane >= j1) ks = vs = 0.f;
+            float top = max_xor32(max_xor16(fmaxf(vs, 0.f)));
+            top = fmaxf(top, dpp<0xB1>(top));
+            top = fmaxf(top, dpp<0x4E>(top));
+            top = fmaxf(top, dpp<0x141>(top));
+            top = fmaxf(top, dpp<0x140>(top));
+            const int e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) : -126;
+            const int En = uniform(max(E, e));
+            efac = __builtin_amdgcn_ldexpf(1.f, E - En);
+            E = En;
+            s_k[lane] = ks * to_log2;
+            s_v[lane] = __builtin_amdgcn_ldexpf(vs, kProbBits - En);
+        }
+#pragma unroll
+        for (int h = 0; h < SUB; ++h)
+#pragma unroll
+            for (int i = 0; i < VL; ++i) {
+                const int off = i * 1024 + lane * 16;
+                const int r = 16 * h + off / ROW, cb = off % ROW;
+                *reinterpret_cast<u32x4*>(kt + r * ROW + piece(r, cb >> 4) * 16) = T.k[h][i];
+                if constexpr (Q8) *reinterpret_cast<u32x4*>(vt + r * ROW + piece(r, cb >> 4) * 16) = T.v[h][i];
+                else *reinterpret_cast<u32x4*>(vt + r * ROW + vseg(r, cb >> 5) * 32 + (cb & 31)) = T.v[h][i];
+            }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
+        f32x4 S[R][SUB];
+#pragma unroll
+        for (int h = 0; h < SUB; ++h) {
+            const int r = 16 * h + n16;
+            f16x8v ka[KD];
+            if constexpr (Q8) {
+#pragma unroll
+                for (int j = 0; j < KD / 2; ++j) {
+                    const u32x4 c = *reinterpret_cast<const u32x4*>(kt + r * ROW + piece(r, g4 + 4 * j) * 16);
+                    ka[2 * j] = codes_to_f16x8<CT>(u32x2{c[0], c[1]});
+                    ka[2 * j + 1] = codes_to_f16x8<CT>(u32x2{c[2], c[3]});
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < KD; ++j)
+                    ka[j] = *reinterpret_cast<const f16x8v*>(kt + r * ROW + piece(r, g4 + 4 * j) * 16);
+            }
+#pragma unroll
+            for (int a = 0; a < R; ++a) {
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < KD; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[j], qb[a][j], acc, 0, 0, 0);
+                S[a][h] = acc;
+            }
+        }
+        f32x4 vf[SUB];
+#pragma unroll
+        for (int h = 0; h < SUB; ++h) {
+            f32x4 kf;
+            if constexpr (Q8) {
+                kf = *reinterpret_cast<const f32x4*>(s_k + 16 * h + 4 * g4);
+                vf[h] = *reinterpret_cast<const f32x4*>(s_v + 16 * h + 4 * g4);
+            }
+#pragma unroll
+            for (int a = 0; a < R; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[a][h][r] *= Q8 ? kf[r] : to_log2;
+        }
+        f16x8v pa[R][SUB / 2];
+        float cr[R][4];
+#pragma unroll
+        for (int a = 0; a < R; ++a) {
+            if (cap) {
+#pragma unroll
+                for (int i = 0; i < 4 * SUB; ++i)
+                    S[a][i >> 2][i & 3] = capped(S[a][i >> 2][i & 3], 1.f, p.cap_log2);
+            }
+            bool ok[4 * SUB];
+            float mx = -FLT_MAX;
+#pragma unroll
+            for (int i = 0; i < 4 * SUB; ++i) {
+                const int key = t0 + 16 * (i >> 2) + 4 * g4 + (i & 3);
+                ok[i] = FULL || (key < j1 && key <= pos[a] && (p.window <= 0 || key > pos[a] - p.window));
+                mx = ok[i] ? fmaxf(mx, S[a][i >> 2][i & 3]) : mx;
+            }
+            mx = max_xor32(max_xor16(mx));
+            const float mn = fmaxf(m[a], mx), corr = fast_exp2(m[a] - mn);
+            const float ref = Q8 ? mn : mn - (float)kProbBits;
+            float ps = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4 * SUB; ++i) {
+                const float e = ok[i] ? fast_exp2(S[a][i >> 2][i & 3] - ref) : 0.f;
+                ps += e;
+                const float pv = !Q8 ? e : (ok[i] ? e * vf[i >> 2][i & 3] : 0.f);
+                pa[a][i >> 3][i & 7] = (_Float16)pv;
+            }
+            l[a] = __builtin_fmaf(l[a], corr, ps);
+            m[a] = mn;
+            const float oc = Q8 ? corr * efac : corr;
+            // row 4 g + r of the output belongs to the lane that holds row 4 g + r of the scores
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                cr[a][r] = __int_as_float(__builtin_amdgcn_ds_bpermute((4 * g4 + r) << 2, __float_as_int(oc)));
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            f16x8v vv[SUB / 2];
+#pragma unroll
+            for (int s = 0; s < SUB / 2; ++s) {
+                if constexpr (Q8) {
+                    const int j = n16 >> 1, r = 32 * s + (j < 4 ? 4 * g4 + j : 12 + 4 * g4 + j);
+                    vv[s] = codes_to_f16x8<CT>(ds_read_tr8(vt + r * ROW + piece(r, nt) * 16 + 8 * (n16 & 1)));
+                } else {
+                    const int r = 32 * s + 4 * g4 + (n16 >> 2), cb = 8 * (n16 & 3);
+                    const s16x4v lo = ds_read_tr16(vt + r * ROW + vseg(r, nt) * 32 + cb);
+                    const s16x4v hi = ds_read_tr16(vt + (r + 16) * ROW + vseg(r + 16, nt) * 32 + cb);
+                    vv[s] = __builtin_bit_cast(f16x8v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < R; ++a) {
+                f32x4 pv = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < SUB / 2; ++s) pv = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa[a][s], vv[s], pv, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) O[a][nt][r] = __builtin_fmaf(O[a][nt][r], cr[a][r], pv[r]);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
+    };
+    const int plast = u.pos0 + u.ntok - 1;
+    auto step = [&](int k, Tile& T) {
+        const int t0 = j0 + (wave + W * k) * KT;
+        if (t0 + KT <= j1 && t0 + KT - 1 <= u.pos0 && (p.window <= 0 || t0 > plast - p.window)) consume(k, T, std::true_type{});
+        else consume(k, T, std::false_type{});
+    };
+    // the next tile (its ids a new set of 64 subtiles now and then) while this one is computed
+    auto next = [&](int k, Tile& T) {
+        if (((SUB * k) & (kWave - 1)) == 0) load_ids(SUB * k);
+        issue(k, T);
+    };
+    for (int k = 0; k < kmax; k += 2) {
+        if (k + 1 < kmax) next(k + 1, B);
+        step(k, A);
+        if (k + 1 >= kmax) break;
+        if (k + 2 < kmax) next(k + 2, A);
+        step(k + 1, B);
+    }
+
+    // the waves' (m, l, O) through LDS, each over its own tiles; rows of dims are then summed
+    static_assert(16 * R * D * 4 <= 2 * Sh::kTile, "partials fit the tiles");
+    const int nwa = min(W, ntiles);
+    __shared__ float s_ml[Sh::W][16 * R][3];
+    __shared__ int s_bad[Sh::W];
+    if (lane == 0) s_bad[wave] = bad;
+    if (wave < nwa) {
+        float* acc = reinterpret_cast<float*>(kt);
+#pragma unroll
+        for (int a = 0; a < R; ++a) {
+            const float lt = sum_xor32(sum_xor16(l[a]));
+            if (lane < 16) {
+                s_ml[wave][16 * a + lane][0] = m[a];
+                s_ml[wave][16 * a + lane][1] = lt;
+                s_ml[wave][16 * a + lane][2] = Q8 ? __builtin_amdgcn_ldexpf(1.f, E - kProbBits) : 1.f;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[(16 * a + 4 * g4 + r) * D + n16 + 16 * nt] = O[a][nt][r];
+        }
+    }
+    __syncthreads();
+    int any_bad = 0;
+    if constexpr (!Q8) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) any_bad |= s_bad[w];
+    }
+    for (int idx = threadIdx.x; idx < u.rows * (D / 4); idx += W * kWave) {
+        const int r = idx / (D / 4), d = idx % (D / 4) * 4;
+        float M = -FLT_MAX;
+        for (int w = 0; w < nwa; ++w) M = fmaxf(M, s_ml[w][r][0]);
+        float lt = 0.f;
+        f32x4 at = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < nwa; ++w) {
+            const float wl = fast_exp2(s_ml[w][r][0] - M), wa = wl * s_ml[w][r][2];
+            lt = __builtin_fmaf(wl, s_ml[w][r][1], lt);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(lds + w * Sh::kWaveBytes + (r * D + d) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) at[e] = __builtin_fmaf(wa, x[e], at[e]);
+        }
+        if (any_bad) at = add_seen_nonfinite<D>(p, u, at, u.pos0 + r / u.hn, d);
+        if (u.nc == 1) {
+            const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+            f16x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (_Float16)(at[e] * inv);
+            *reinterpret_cast<f16x4*>(p.out + chunk_row(p, u, r, D) + d) = o;
+        } else {
+            const size_t rec = (size_t)u.hk * p.n_records + u.rec0 + (size_t)u.c * u.rows + r;
+            *reinterpret_cast<f32x4*>(p.part_acc + rec * D + d) = at;
+            if (d == 0) {
+                p.part_ml[rec * 2] = M;
+                p.part_ml[rec * 2 + 1] = lt;
+            }
+        }
+    }
+}
+
+template <int D, int CT>
+__global__ __launch_bounds__((StreamShape<D, CT>::W * kWave)) void chunk_stream_kernel(ChunkParams p) {
+    __shared__ __attribute__((aligned(16))) char lds[StreamShape<D, CT>::kBytes];
+    ChunkUnit u;
+    if (!chunk_unit(p, u) || u.kind != kKindRows) return;
+    if (u.rows <= 16) stream_unit<D, CT, 1>(p, u, lds);
+    else if (u.rows <= 32) stream_unit<D, CT, 2>(p, u, lds);
+}
+
 // Partial rows of the units with nc > 1 as output rows: out = sum_c 2^(m_c - M) acc_c / sum_c
 // 2^(m_c - M) l_c.  The workgroup of a unit's first chunk takes its rows, a wave one at a time.
 template <int D>
