@@ -45,7 +45,7 @@ constexpr int kChunkKeys = 1024;
 void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N, int Hq, int Hkv, int D, int BLOCK,
                 int window, std::vector<PlanUnit>& units, long long& records) {
     const int group = Hq / Hkv;
-    const int kRowsPerUnit = matrix_path(D, BLOCK) ? 32 : 16;
+    constexpr int kRowsPerUnit = 16;
     std::vector<Tile> tiles;
     long long row = 0, tab = 0;
     for (int s = 0; s < N; ++s) {

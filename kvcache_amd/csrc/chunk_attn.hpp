@@ -294,10 +294,10 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
     };
     auto vseg = [](int r, int seg) { return seg ^ (D == 64 ? (r >> 1) & 3 : r & 7); };
 
-    Tile A, B;
+    Tile T;
     if (kmax > 0) {
         load_ids(0);
-        issue(0, A);
+        issue(0, T);
     }
     // q as the B operand: lane l holds row l % 16; 8-bit: dims 64 j + 16 g + 8 e .. + 7 in step 2 j + e
     f16x8v qb[R][KD];
@@ -324,9 +324,10 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
         for (int nt = 0; nt < NT; ++nt) O[a][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
+    auto fence = [] { asm volatile("" ::: "memory"); };
     bool bad = false;  // this wave cleared elements of V in tiles that some row does not see whole
     // FULL: every key of the tile is seen by every row
-    auto consume = [&](int k, Tile& T, auto full_tag) {
+    auto consume = [&](int k, auto full_tag) {
         constexpr bool FULL = decltype(full_tag)::value;
         const int t0 = j0 + (wave + W * k) * KT;
         if constexpr (!Q8 && !FULL) {
@@ -367,11 +368,18 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
             }
         __builtin_amdgcn_wave_barrier();
         asm volatile("" ::: "memory");
+        // the next tile is on its way while this one is computed (its ids a new set of 64
+        // subtiles now and then)
+        if (k + 1 < kmax) {
+            if (((SUB * (k + 1)) & (kWave - 1)) == 0) load_ids(SUB * (k + 1));
+            issue(k + 1, T);
+        }
         f32x4 S[R][SUB];
 #pragma unroll
         for (int h = 0; h < SUB; ++h) {
             const int r = 16 * h + n16;
             f16x8v ka[KD];
+            fence();
             if constexpr (Q8) {
 #pragma unroll
                 for (int j = 0; j < KD / 2; ++j) {
@@ -392,14 +400,13 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
                 S[a][h] = acc;
             }
         }
-        f32x4 vf[SUB];
+        // (the fences keep operand reads of later steps from being held in registers through earlier
+        // ones: without them D 64 took 174 registers, two waves a SIMD instead of four)
+        fence();
 #pragma unroll
         for (int h = 0; h < SUB; ++h) {
             f32x4 kf;
-            if constexpr (Q8) {
-                kf = *reinterpret_cast<const f32x4*>(s_k + 16 * h + 4 * g4);
-                vf[h] = *reinterpret_cast<const f32x4*>(s_v + 16 * h + 4 * g4);
-            }
+            if constexpr (Q8) kf = *reinterpret_cast<const f32x4*>(s_k + 16 * h + 4 * g4);
 #pragma unroll
             for (int a = 0; a < R; ++a)
 #pragma unroll
@@ -414,24 +421,31 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
                 for (int i = 0; i < 4 * SUB; ++i)
                     S[a][i >> 2][i & 3] = capped(S[a][i >> 2][i & 3], 1.f, p.cap_log2);
             }
-            bool ok[4 * SUB];
+            // key t0 + 16 h + 4 g + r is seen when low < 16 h + r <= lim
+            const int lim = min(pos[a], j1 - 1) - t0 - 4 * g4;
+            const int low = (p.window > 0 ? pos[a] - p.window : -1) - t0 - 4 * g4;
+            auto seen = [&](int i) {
+                const int c = 16 * (i >> 2) + (i & 3);
+                return FULL || (c <= lim && c > low);
+            };
             float mx = -FLT_MAX;
 #pragma unroll
-            for (int i = 0; i < 4 * SUB; ++i) {
-                const int key = t0 + 16 * (i >> 2) + 4 * g4 + (i & 3);
-                ok[i] = FULL || (key < j1 && key <= pos[a] && (p.window <= 0 || key > pos[a] - p.window));
-                mx = ok[i] ? fmaxf(mx, S[a][i >> 2][i & 3]) : mx;
-            }
+            for (int i = 0; i < 4 * SUB; ++i) mx = seen(i) ? fmaxf(mx, S[a][i >> 2][i & 3]) : mx;
             mx = max_xor32(max_xor16(mx));
             const float mn = fmaxf(m[a], mx), corr = fast_exp2(m[a] - mn);
             const float ref = Q8 ? mn : mn - (float)kProbBits;
             float ps = 0.f;
+            fence();
 #pragma unroll
-            for (int i = 0; i < 4 * SUB; ++i) {
-                const float e = ok[i] ? fast_exp2(S[a][i >> 2][i & 3] - ref) : 0.f;
-                ps += e;
-                const float pv = !Q8 ? e : (ok[i] ? e * vf[i >> 2][i & 3] : 0.f);
-                pa[a][i >> 3][i & 7] = (_Float16)pv;
+            for (int h = 0; h < SUB; ++h) {
+                f32x4 vf;
+                if constexpr (Q8) vf = *reinterpret_cast<const f32x4*>(s_v + 16 * h + 4 * g4);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float e = seen(4 * h + r) ? fast_exp2(S[a][h][r] - ref) : 0.f;
+                    ps += e;
+                    pa[a][h >> 1][4 * (h & 1) + r] = (_Float16)(!Q8 ? e : seen(4 * h + r) ? e * vf[r] : 0.f);
+                }
             }
             l[a] = __builtin_fmaf(l[a], corr, ps);
             m[a] = mn;
@@ -443,6 +457,7 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            if ((nt & 1) == 0) fence();
             f16x8v vv[SUB / 2];
 #pragma unroll
             for (int s = 0; s < SUB / 2; ++s) {
@@ -469,22 +484,21 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
         asm volatile("" ::: "memory");
     };
     const int plast = u.pos0 + u.ntok - 1;
-    auto step = [&](int k, Tile& T) {
-        const int t0 = j0 + (wave + W * k) * KT;
-        if (t0 + KT <= j1 && t0 + KT - 1 <= u.pos0 && (p.window <= 0 || t0 > plast - p.window)) consume(k, T, std::true_type{});
-        else consume(k, T, std::false_type{});
+    // tiles that every row sees whole, between those of the window's edge and of the causal one
+    // (loops of their own: one loop with both forms kept the registers of either through both)
+    auto tiles_to = [&](int keys) {  // this wave's tiles that begin before j0 + keys
+        const int n = max(0, (keys + KT - 1) / KT);
+        return min(kmax, n > wave ? (n - wave + W - 1) / W : 0);
     };
-    // the next tile (its ids a new set of 64 subtiles now and then) while this one is computed
-    auto next = [&](int k, Tile& T) {
-        if (((SUB * k) & (kWave - 1)) == 0) load_ids(SUB * k);
-        issue(k, T);
-    };
-    for (int k = 0; k < kmax; k += 2) {
-        if (k + 1 < kmax) next(k + 1, B);
-        step(k, A);
-        if (k + 1 >= kmax) break;
-        if (k + 2 < kmax) next(k + 2, A);
-        step(k + 1, B);
+    const int whole = min(u.pos0 + 1, j1) - j0;  // keys that every row's position reaches
+    const int kf0 = p.window > 0 ? tiles_to(plast - p.window + 1 - j0) : 0;
+    const int kf1 = max(kf0, tiles_to(whole / KT * KT));
+    int k = 0;
+    for (int end = kf0;;) {
+        for (; k < end; ++k) consume(k, std::false_type{});
+        if (end == kmax) break;
+        for (; k < kf1; ++k) consume(k, std::true_type{});
+        end = kmax;
     }
 
     // the waves' (m, l, O) through LDS, each over its own tiles; rows of dims are then summed
@@ -547,41 +561,74 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
 }
 
 template <int D, int CT>
-__global__ __launch_bounds__((StreamShape<D, CT>::W * kWave)) void chunk_stream_kernel(ChunkParams p) {
+__global__ __launch_bounds__((StreamShape<D, CT>::W * kWave), (D == 64 ? 4 : 2)) void chunk_stream_kernel(ChunkParams p) {
     __shared__ __attribute__((aligned(16))) char lds[StreamShape<D, CT>::kBytes];
     ChunkUnit u;
     if (!chunk_unit(p, u) || u.kind != kKindRows) return;
     if (u.rows <= 16) stream_unit<D, CT, 1>(p, u, lds);
-    else if (u.rows <= 32) stream_unit<D, CT, 2>(p, u, lds);
 }
 
 // Partial rows of the units with nc > 1 as output rows: out = sum_c 2^(m_c - M) acc_c / sum_c
-// 2^(m_c - M) l_c.  The workgroup of a unit's first chunk takes its rows, a wave one at a time.
+// 2^(m_c - M) l_c.  A tile's nc units take its rows in turn, one at a time: 256 / (D / 4) chunks
+// side by side (a thread four dims of one), each thread over its chunks, then across them in LDS.
 template <int D>
 __global__ __launch_bounds__(256) void merge_chunks_kernel(ChunkParams p) {
-    constexpr int NJ = (D + kWave - 1) / kWave;
+    constexpr int TD = D / 4, SLOTS = 256 / TD;
+    __shared__ f32x4 s_acc[SLOTS][TD];
+    __shared__ float s_ml[SLOTS][2];
     ChunkUnit u;
-    if (!chunk_unit(p, u) || u.nc == 1 || u.c != 0) return;
-    const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6);
-    for (int r = wave; r < u.rows; r += 4) {
+    if (!chunk_unit(p, u) || u.nc == 1) return;
+    const int slot = threadIdx.x / TD, d = threadIdx.x % TD * 4;
+    const int n = min(SLOTS, u.nc);
+    for (int r = u.c; r < u.rows; r += u.nc) {
         const size_t rec0 = (size_t)u.hk * p.n_records + u.rec0 + r;
-        float M = -FLT_MAX;
-        for (int c = 0; c < u.nc; ++c) M = fmaxf(M, p.part_ml[(rec0 + (size_t)c * u.rows) * 2]);
-        float l = 0.f, acc[NJ];
+        float M = -FLT_MAX, l = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        // four chunks in flight (past the count the last one's again, with weight 0)
+        for (int c = slot; c < u.nc; c += 4 * SLOTS) {
+            float m[4], lc[4];
+            f32x4 a[4];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[j] = 0.f;
-        for (int c = 0; c < u.nc; ++c) {
-            const size_t rec = rec0 + (size_t)c * u.rows;
-            const float w = fast_exp2(p.part_ml[rec * 2] - M);
-            l = __builtin_fmaf(w, p.part_ml[rec * 2 + 1], l);
+            for (int i = 0; i < 4; ++i) {
+                const size_t rec = rec0 + (size_t)min(c + i * SLOTS, u.nc - 1) * u.rows;
+                m[i] = p.part_ml[rec * 2];
+                lc[i] = p.part_ml[rec * 2 + 1];
+                a[i] = *reinterpret_cast<const f32x4*>(p.part_acc + rec * D + d);
+            }
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) acc[j] = __builtin_fmaf(w, p.part_acc[rec * D + min(lane + j * kWave, D - 1)], acc[j]);
+            for (int i = 0; i < 4; ++i) {
+                if (c + i * SLOTS >= u.nc) continue;
+                const float mn = fmaxf(M, m[i]), w0 = fast_exp2(M - mn), w1 = fast_exp2(m[i] - mn);
+                M = mn;
+                l = l * w0 + lc[i] * w1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] = acc[e] * w0 + a[i][e] * w1;
+            }
         }
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-        const size_t o = chunk_row(p, u, r, D);
+        s_acc[slot][threadIdx.x % TD] = acc;
+        if (d == 0) {
+            s_ml[slot][0] = M;
+            s_ml[slot][1] = l;
+        }
+        __syncthreads();
+        if (threadIdx.x < TD) {
+            float Mt = -FLT_MAX, lt = 0.f;
+            f32x4 at = {0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < n; ++i) Mt = fmaxf(Mt, s_ml[i][0]);
+            for (int i = 0; i < n; ++i) {
+                const float w = fast_exp2(s_ml[i][0] - Mt);
+                lt = __builtin_fmaf(w, s_ml[i][1], lt);
+                const f32x4 x = s_acc[i][threadIdx.x];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-            if (lane + j * kWave < D) p.out[o + lane + j * kWave] = (_Float16)(acc[j] * inv);
+                for (int e = 0; e < 4; ++e) at[e] = __builtin_fmaf(w, x[e], at[e]);
+            }
+            const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+            f16x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (_Float16)(at[e] * inv);
+            *reinterpret_cast<f16x4*>(p.out + chunk_row(p, u, r, D) + d) = o;
+        }
+        __syncthreads();
     }
 }
 
