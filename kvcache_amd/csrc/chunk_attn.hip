@@ -1,6 +1,6 @@
 // chunk_attn.hip -- attention of a ragged batch of chunks over a paged cache: the host plan and
 // the launches (kernels in chunk_attn.hpp).
-#include "chunk_attn.hpp"
+#include "chunk_tile.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -40,22 +40,26 @@ struct PlanUnit {
     long long cost;
 };
 
-// The batch as units.
+// The batch as units.  A sequence whose new tokens make more than kStreamRows rows of a KV head
+// is cut into tiles of many rows, others into units of 16.
+constexpr int kStreamRows = 32;
 constexpr int kChunkKeys = 1024;
 void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N, int Hq, int Hkv, int D, int BLOCK,
                 int window, std::vector<PlanUnit>& units, long long& records) {
     const int group = Hq / Hkv;
-    constexpr int kRowsPerUnit = 16;
+    const bool matrix = matrix_path(D, BLOCK);
     std::vector<Tile> tiles;
     long long row = 0, tab = 0;
     for (int s = 0; s < N; ++s) {
         const int nq = q_lens[s], nk = kv_lens[s];
         if (tab_off) tab = tab_off[s];
-        const int hstep = std::min(group, kRowsPerUnit), tstep = std::max(1, kRowsPerUnit / group);
+        const bool many = matrix && (long long)nq * group > kStreamRows;
+        const int cap = !many ? 16 : (long long)nq * group <= 64 ? 64 : (long long)nq * group <= 1024 ? 128 : 256;
+        const int hstep = std::min(group, cap), tstep = std::max(1, cap / group);
         for (int i = 0; i < nq; i += tstep)
             for (int h = 0; h < group; h += hstep) {
-                Tile t{kKindRows, (int)row + i, std::min(tstep, nq - i), nk - nq + i, h, std::min(hstep, group - h), 0, 0,
-                       (int)tab};
+                Tile t{many ? kKindTile : kKindRows, (int)row + i, std::min(tstep, nq - i), nk - nq + i, h,
+                       std::min(hstep, group - h), 0, 0, (int)tab};
                 t.j1 = t.pos0 + t.ntok;
                 t.j0 = window > 0 ? std::max(0, t.pos0 - window + 1) / 64 * 64 : 0;
                 tiles.push_back(t);
@@ -66,7 +70,7 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
     records = 0;
     for (const Tile& t : tiles) {
         const int len = t.j1 - t.j0;
-        int nc = std::max(1, (len + kChunkKeys - 1) / kChunkKeys);
+        int nc = t.kind == kKindTile ? 1 : std::max(1, (len + kChunkKeys - 1) / kChunkKeys);
         const int step = ((len + nc - 1) / nc + 63) / 64 * 64;
         nc = (len + step - 1) / step;
         const int rows = t.ntok * t.hn;
@@ -89,7 +93,9 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
         }
         if (nc > 1) records += (long long)nc * rows;
     }
-    std::stable_sort(units.begin(), units.end(), [](const PlanUnit& a, const PlanUnit& b) { return a.cost > b.cost; });
+    std::stable_sort(units.begin(), units.end(), [](const PlanUnit& a, const PlanUnit& b) {
+        return a.f[kFKind] != b.f[kFKind] ? a.f[kFKind] > b.f[kFKind] : a.cost > b.cost;
+    });
 }
 
 template <typename F>
@@ -104,11 +110,17 @@ int guard_chunk(F&& f) {
 }
 
 template <int D, int CT>
-int launch_chunks_d(const ChunkParams& p, hipStream_t st) {
+int launch_chunks_d(const ChunkParams& p, int n_tiles, hipStream_t st) {
     const dim3 grid((unsigned)((size_t)(p.n_units - 1) * p.Hkv));
     bool done = false;
     if constexpr (D == 64 || D == 128) {
         if (matrix_path(D, p.block)) {
+            if (n_tiles > 0) {  // the list's tiles come first
+                const dim3 tgrid((unsigned)((size_t)std::min(n_tiles, p.n_units - 1) * p.Hkv));
+                hipLaunchKernelGGL((chunk_tile_kernel<D, CT>), tgrid, dim3(8 * kWave), 0, st, p);
+                const int rc = hip_check(hipGetLastError(), "chunk attention launch");
+                if (rc) return rc;
+            }
             hipLaunchKernelGGL((chunk_stream_kernel<D, CT>), grid, dim3(StreamShape<D, CT>::W * kWave), 0, st, p);
             done = true;
         }
@@ -121,10 +133,10 @@ int launch_chunks_d(const ChunkParams& p, hipStream_t st) {
 }
 
 template <int D>
-int launch_chunks(const ChunkParams& p, int kv_dtype, hipStream_t st) {
-    if (kv_dtype == KVC_F16) return launch_chunks_d<D, kCacheF16>(p, st);
-    if (kv_dtype == KVC_I8) return launch_chunks_d<D, kCacheI8>(p, st);
-    return launch_chunks_d<D, kCacheE4M3>(p, st);
+int launch_chunks(const ChunkParams& p, int n_tiles, int kv_dtype, hipStream_t st) {
+    if (kv_dtype == KVC_F16) return launch_chunks_d<D, kCacheF16>(p, n_tiles, st);
+    if (kv_dtype == KVC_I8) return launch_chunks_d<D, kCacheI8>(p, n_tiles, st);
+    return launch_chunks_d<D, kCacheE4M3>(p, n_tiles, st);
 }
 
 }  // namespace
@@ -223,10 +235,10 @@ int kvc_paged_chunk_attn(const void* q, void* out, const void* k_pool, const voi
         }
         const hipStream_t st = (hipStream_t)stream;
         switch (D) {
-            case 32: return launch_chunks<32>(p, kv_dtype, st);
-            case 64: return launch_chunks<64>(p, kv_dtype, st);
-            case 128: return launch_chunks<128>(p, kv_dtype, st);
-            default: return launch_chunks<256>(p, kv_dtype, st);
+            case 32: return launch_chunks<32>(p, n_tiles, kv_dtype, st);
+            case 64: return launch_chunks<64>(p, n_tiles, kv_dtype, st);
+            case 128: return launch_chunks<128>(p, n_tiles, kv_dtype, st);
+            default: return launch_chunks<256>(p, n_tiles, kv_dtype, st);
         }
     });
 }

@@ -1,0 +1,426 @@
+// chunk_tile.hpp -- chunk attention of many rows on the matrix cores (head_dim 64 / 128).
+//
+// A workgroup of 8 waves takes 32 QG rows (token, head) of one KV head, QG groups of 32 rows
+// times KS = 8 / QG key streams.  Keys come in sets of 128, stream ks of a set taking its
+// 128 / KS keys.  Wave w brings rows 16 w .. + 15 of a set (one block id, whole rows, rows past
+// the end read as zero through the descriptor) into registers while the set before is computed,
+// then, as fp16, into the other half of the LDS buffer; one barrier per set.
+//
+//   8-bit rows become fp16 on their way into LDS, once for all rows of the workgroup: K times
+//     its scale and the factor to log2 units, V times its scale, each product rounded once (what
+//     an fp16 cache would hold; values beyond fp16's range, 65504, become Inf).
+//   S^T[key][row] = K Q^T with v_mfma_f32_32x32x16_f16: a lane holds 16 scores of ONE row
+//     (column l % 32), so a row's maximum needs one exchange with lane l ^ 32.  8-bit caches
+//     start the accumulator at kBias - reference, so the products' sum is the exponent itself.
+//   softmax: p = 2^(s - reference + kBias), fp32, then fp16.  The reference lags: it moves to the
+//     row's maximum when a score passes it by more than 2^kLag (and at a row's first key), so p
+//     is at most 2^15, fp16 keeps all its bits down to 2^-21 of the largest, and O is rescaled a
+//     few times per row instead of nearly every tile.  The sum is taken over the rounded
+//     probabilities (two a v_dot2), the ones O is made of.
+//   O^T[dim][row] += V^T P^T: the lane's own probabilities are the operand up to the order of
+//     keys, and V^T is read back in that order with the transposing LDS read.
+//
+// LDS: K rows as 16-byte chunks XOR-permuted by the row, V rows as 32-byte segments permuted by
+// the row, so that neither operand read meets a bank twice.
+#pragma once
+#include "chunk_attn.hpp"
+
+namespace kvc {
+namespace {
+
+constexpr float kBias = 7.f, kLag = 8.f;
+
+// Sixteen codes times s as fp16, each rounded once.  int8: the fp16 1024 + (c + 128) comes from a
+// byte permutation, and one fma takes 1152 s off again; s has 20 bits (row_factor), so that 1152 s
+// is exact.
+template <int CT>
+__device__ __forceinline__ void scaled_f16(u32x4 c, float s, u32x4 (&out)[2]) {
+    const float off = CT == kCacheI8 ? -1152.f * s : 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f16x2 a, b;
+        if constexpr (CT == kCacheI8) {
+            const unsigned x = c[w] ^ 0x80808080u;
+            a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u));
+            b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u));
+        } else {
+            codes_to_f16<CT>(c[w], a, b);
+        }
+        f16x4 y;
+        y[0] = (_Float16)__builtin_fmaf((float)a[0], s, off);
+        y[1] = (_Float16)__builtin_fmaf((float)a[1], s, off);
+        y[2] = (_Float16)__builtin_fmaf((float)b[0], s, off);
+        y[3] = (_Float16)__builtin_fmaf((float)b[1], s, off);
+        const u32x2 z = __builtin_bit_cast(u32x2, y);
+        out[w >> 1][2 * (w & 1)] = z[0];
+        out[w >> 1][2 * (w & 1) + 1] = z[1];
+    }
+}
+
+__device__ __forceinline__ float row_factor(float s) { return __uint_as_float(__float_as_uint(s) & 0xFFFFFFF0u); }
+
+// add_seen_nonfinite (chunk_attn.hpp) of the elements as tile_unit stages them.
+template <int D, int CT>
+__device__ __forceinline__ f32x4 add_seen_nonfinite_q8(const ChunkParams& p, const ChunkUnit& u, f32x4 acc, int pos, int d0) {
+    const int bsh = __builtin_ctz((unsigned)p.block);
+    const int first = max(u.j0, p.window > 0 ? pos - p.window + 1 : 0), last = min(u.j1 - 1, pos);
+    for (int j = first; j <= last; ++j) {
+        const int id = p.table[min(u.tab + (j >> bsh), p.table_len - 1)];
+        const size_t row = (((size_t)(unsigned)(id * p.Hkv + u.hk)) << bsh) + (j & (p.block - 1));
+        f16x2 a, b;
+        codes_to_f16<CT>(*reinterpret_cast<const unsigned*>(static_cast<const char*>(p.v) + row * D + d0), a, b);
+        const float s = row_factor(p.scales[row * 2 + 1]);
+        const f16x4 v = {(_Float16)((float)a[0] * s), (_Float16)((float)a[1] * s), (_Float16)((float)b[0] * s),
+                         (_Float16)((float)b[1] * s)};
+        const u16x4 bits = __builtin_bit_cast(u16x4, v);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (nonfinite(bits[r])) acc[r] += (float)v[r];
+    }
+    return acc;
+}
+
+constexpr int kSetKeys = 128;  // keys of an LDS set: 16 rows for each of 8 waves
+
+template <int D>
+struct TileLds {
+    char kv[2][2][kSetKeys * D * 2];  // [half][K / V]
+};
+
+template <int D, int CT, int QG>
+__device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit& u, TileLds<D>& lds) {
+    constexpr bool Q8 = CT != kCacheF16;
+    constexpr int W = 8;
+    constexpr int SRC = D * kCodeBytes<CT>;  // bytes of a cached row
+    constexpr int ROW = D * 2;               // ... of a row in LDS
+    constexpr int KS = W / QG;               // key streams
+    constexpr int KT = kSetKeys / KS;        // keys per stream and set
+    constexpr int NS = KT / 32;              // 32-key subtiles
+    constexpr int KD = D / 16;               // MFMA k steps over the head dimension
+    constexpr int DT = D / 32;               // 32-dim output tiles
+    constexpr int VL = 16 * SRC / 1024;      // wave loads per 16 rows
+    constexpr int kSetBytes = kSetKeys * ROW;
+    static_assert(KS == 1 || KS * QG * 32 * D * 4 <= 2 * 2 * kSetBytes, "partials fit the tile buffers");
+    __shared__ float s_ml[KS][QG][32][2];
+    __shared__ int s_bad[W];
+
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = uniform(threadIdx.x >> 6);
+    const int qg = wave % QG, ks = wave / QG;
+    const int l32 = lane & 31, h = lane >> 5;
+    const int j0 = u.j0, j1 = u.j1;
+    const int nsets = (j1 - j0 + kSetKeys - 1) / kSetKeys;
+    const int bsh = __builtin_ctz((unsigned)p.block), bmask = p.block - 1;
+    const char* kb = static_cast<const char*>(p.k);
+    const char* vb = static_cast<const char*>(p.v);
+    const bool cap = p.cap_log2 > 0.f;
+    const float to_log2 = cap ? p.cap_in : p.scale_log2;
+
+    // this wave's rows of set s; block ids one set per lane, 64 sets at a time
+    auto first_tok = [&](int s) { return j0 + s * kSetKeys + 16 * wave; };
+    int ids = 0;
+    auto load_ids = [&](int s) {
+        ids = p.table[min(u.tab + (min(first_tok(s + lane), j1 - 1) >> bsh), p.table_len - 1)];
+    };
+    u32x4 rk[VL], rv[VL];
+    f32x2 sc[VL];
+    int i_rows = 0;
+    size_t i_row = 0;
+    auto issue = [&](int s) {
+        const int t = first_tok(s);
+        const int id = __builtin_amdgcn_readlane(ids, s & (kWave - 1));
+        int rows = max(j1 - t, 0);
+        asm("" : "+s"(rows));
+        i_rows = min(rows, 16);
+        i_row = (((size_t)(unsigned)(id * p.Hkv + u.hk)) << bsh) + (t & bmask);
+        const __amdgpu_buffer_rsrc_t kr = tile_rsrc(kb + i_row * SRC, i_rows * SRC), vr = tile_rsrc(vb + i_row * SRC, i_rows * SRC);
+#pragma unroll
+        for (int i = 0; i < VL; ++i) rk[i] = buffer_load16(kr, i * 1024 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < VL; ++i) rv[i] = buffer_load16(vr, i * 1024 + lane * 16);
+        if constexpr (Q8) {  // (rows past the end read as scale 0)
+            const __amdgpu_buffer_rsrc_t sr = tile_rsrc(p.scales + i_row * 2, i_rows * 8);
+#pragma unroll
+            for (int i = 0; i < VL; ++i)
+                sc[i] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(sr, (i * 1024 + lane * 16) / SRC * 8, 0, 0));
+        }
+    };
+    auto kchunk = [](int r, int ch) { return ch ^ (r & 7); };
+    auto vseg = [](int r, int seg) { return seg ^ (D == 64 ? (r >> 1) & 3 : r & 7); };
+    bool bad = false;  // this wave cleared elements of V in sets that some row does not see whole
+    auto store = [&](int half, bool edge) {
+        char* kd = lds.kv[half][0];
+        char* vd = lds.kv[half][1];
+        if constexpr (Q8) {
+#pragma unroll
+            for (int i = 0; i < VL; ++i) {
+                const int off = i * 1024 + lane * 16;
+                const int r = 16 * wave + off / SRC, c = off % SRC / 8;  // first of two 16-byte chunks
+                u32x4 x[2];
+                scaled_f16<CT>(rk[i], row_factor(sc[i][0] * to_log2), x);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) *reinterpret_cast<u32x4*>(kd + r * ROW + kchunk(r, c + e) * 16) = x[e];
+                scaled_f16<CT>(rv[i], row_factor(sc[i][1]), x);
+                if (edge && any_nonfinite(x)) {
+                    clear_nonfinite(x);
+                    bad = true;
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) *reinterpret_cast<u32x4*>(vd + r * ROW + vseg(r, c >> 1) * 32 + e * 16) = x[e];
+            }
+        } else {
+            if (edge && any_nonfinite(rv)) {
+                clear_nonfinite(rv);
+                bad = true;
+            }
+#pragma unroll
+            for (int i = 0; i < VL; ++i) {
+                const int off = i * 1024 + lane * 16;
+                const int r = 16 * wave + off / ROW, cb = off % ROW;
+                *reinterpret_cast<u32x4*>(kd + r * ROW + kchunk(r, cb >> 4) * 16) = rk[i];
+                *reinterpret_cast<u32x4*>(vd + r * ROW + vseg(r, cb >> 5) * 32 + (cb & 31)) = rv[i];
+            }
+        }
+    };
+
+    load_ids(0);
+    issue(0);
+    // q as the B operand: lane l holds row 32 qg + l % 32, dims 16 d + 8 (l / 32) .. + 7
+    const int row = 32 * qg + l32, rowc = min(row, u.rows - 1);
+    const int pos = u.pos0 + rowc / u.hn;
+    f16x8v qb[KD];
+    {
+        const _Float16* q = p.q + chunk_row(p, u, rowc, D) + 8 * h;
+#pragma unroll
+        for (int d = 0; d < KD; ++d) qb[d] = *reinterpret_cast<const f16x8v*>(q + 16 * d);
+    }
+    const int wfirst = u.pos0 + min(32 * qg, u.rows - 1) / u.hn;      // positions of the wave's rows
+    const int wlast = u.pos0 + min(32 * qg + 31, u.rows - 1) / u.hn;
+    const int plast = u.pos0 + u.ntok - 1;
+
+    float ref = 0.f, l = 0.f;    // reference of p; sum of the lane's own keys
+    float thr = -FLT_MAX;        // a relative score above it moves the reference (none met yet: any)
+    f32x16 O[DT], C;             // C: what the score accumulator starts from
+#pragma unroll
+    for (int i = 0; i < 16; ++i) C[i] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) O[dt][i] = 0.f;
+    const bool direct = Q8 && !cap;  // the accumulator is the relative score
+    if (direct) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) C[i] = kBias;
+    }
+
+    int ka[4], va[DT];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) ka[d] = ks * KT * ROW + l32 * ROW + kchunk(l32, 2 * d + h) * 16;
+    const int vr = 4 * h + ((lane & 15) >> 2);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+        va[dt] = kSetBytes + ks * KT * ROW + vr * ROW + vseg(vr, 2 * dt + ((lane >> 4) & 1)) * 32 + 8 * (lane & 3);
+    const char* base = &lds.kv[0][0][0];
+
+    auto compute = [&](int half, int t0, auto masked_tag) {
+        constexpr bool MASKED = decltype(masked_tag)::value;
+        const char* buf = base + half * (2 * kSetBytes);
+        auto scores = [&](int n) {
+            f32x16 S = C;
+#pragma unroll
+            for (int d = 0; d < KD; ++d) {
+                const f16x8v a = *reinterpret_cast<const f16x8v*>(buf + ka[d & 3] + 32 * n * ROW + (d >> 2) * 128);
+                S = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qb[d], S, 0, 0, 0);
+            }
+            return S;
+        };
+        // S[i] is key t0 + 32 n + 8 (i / 4) + 4 h + i % 4, seen when low < 32 n + 8 (i / 4) + i % 4 <= lim
+        const int lim = min(pos, j1 - 1) - t0 - 4 * h;
+        const int low = (p.window > 0 ? pos - p.window : -1) - t0 - 4 * h;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            f32x16 S = scores(n);
+            auto seen = [&](int i) {
+                const int c = 32 * n + 8 * (i >> 2) + (i & 3);
+                return !MASKED || (c <= lim && c > low);
+            };
+            if (!direct) {
+                const float off = kBias - ref;
+                if (cap) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) S[i] = capped(Q8 ? S[i] : S[i] * to_log2, 1.f, p.cap_log2) + off;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) S[i] = __builtin_fmaf(S[i], to_log2, off);
+                }
+            }
+            float mx = -FLT_MAX;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = seen(i) ? fmaxf(mx, S[i]) : mx;
+            if (__any(mx > thr)) {
+                mx = max_xor32(mx);
+                const bool move = mx > thr;
+                const float by = move ? mx - kBias : 0.f;
+                const float corr = move && thr > -FLT_MAX ? fast_exp2(-by) : 1.f;
+                ref += by;
+                thr = move ? kBias + kLag : thr;
+                l *= corr;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) S[i] -= by;
+                if (direct) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) C[i] = kBias - ref;
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) O[dt][i] *= corr;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f16x8v pb;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float e = fast_exp2(S[8 * t + j]);
+                    pb[j] = (_Float16)(seen(8 * t + j) ? e : 0.f);
+                }
+                const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
+                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb, pb, 0, 1), one, l, false);
+                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb, pb, 2, 3), one, l, false);
+                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb, pb, 4, 5), one, l, false);
+                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb, pb, 6, 7), one, l, false);
+                // V^T operand: k slots (h, j) are keys 32 n + 16 t + 8 (j / 4) + 4 h + j % 4, of dim
+                // 32 dt + l % 32; two transposing reads of four keys each (16 lanes address four
+                // rows of 16 dims: lane i row i / 4, dims 4 (i % 4) .. + 3)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const char* vt = buf + va[dt] + (32 * n + 16 * t) * ROW;
+                    const s16x4v lo = ds_read_tr16(vt), hi = ds_read_tr16(vt + 8 * ROW);
+                    const f16x8v a = __builtin_bit_cast(f16x8v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                    O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pb, O[dt], 0, 0, 0);
+                }
+            }
+        }
+    };
+
+    // sets that every row sees whole: [f0, f1); before them the window's edge, after them the causal one
+    const int f0 = p.window > 0 ? min(nsets, max(0, plast - p.window + 1 - j0 + kSetKeys - 1) / kSetKeys) : 0;
+    const int f1 = max(f0, (min(u.pos0 + 1, j1) - j0) / kSetKeys);
+    auto whole = [&](int s) { return s >= f0 && s < f1; };
+    store(0, !whole(0));
+    issue(1);
+    // one set: the next one from its registers into the other half of the buffer, the one after
+    // that into flight, then this one's arithmetic
+    auto set = [&](int s, auto masked_tag) {
+        __syncthreads();
+        store((s + 1) & 1, decltype(masked_tag)::value || s + 1 >= f1);
+        if (((s + 2) & (kWave - 1)) == 0) load_ids(s + 2);
+        issue(s + 2);  // (sets past the end read nothing: zero-size descriptors)
+        const int t0 = j0 + s * kSetKeys + ks * KT;
+        if (!decltype(masked_tag)::value ||
+            (32 * qg < u.rows && t0 <= wlast && t0 < j1 && (p.window <= 0 || t0 + KT > wfirst - p.window + 1)))
+            compute(s & 1, t0, masked_tag);
+    };
+    // (loops of their own: one loop with both forms copied O between them in every set)
+    int s = 0;
+    for (int end = f0;;) {
+        for (; s < end; ++s) set(s, std::true_type{});
+        if (end == nsets) break;
+        for (; s < f1; ++s) set(s, std::false_type{});
+        end = nsets;
+    }
+    l = sum_xor32(l);
+    const float m = thr > -FLT_MAX ? ref : -FLT_MAX;
+
+    auto write = [&](int r, int d0, f32x4 acc, float M, float lt) {
+        if (u.nc == 1) {
+            const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+            f16x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (_Float16)(acc[e] * inv);
+            *reinterpret_cast<f16x4*>(p.out + chunk_row(p, u, r, D) + d0) = o;
+        } else {
+            const size_t rec = (size_t)u.hk * p.n_records + u.rec0 + (size_t)u.c * u.rows + r;
+            *reinterpret_cast<f32x4*>(p.part_acc + rec * D + d0) = acc;
+            if (d0 == 0) {
+                p.part_ml[rec * 2] = M;
+                p.part_ml[rec * 2 + 1] = lt;
+            }
+        }
+    };
+    auto add_bad = [&](f32x4 acc, int d0) {
+        if constexpr (Q8) return add_seen_nonfinite_q8<D, CT>(p, u, acc, pos, d0);
+        else return add_seen_nonfinite<D>(p, u, acc, pos, d0);
+    };
+    if (lane == 0) s_bad[wave] = bad;
+    __syncthreads();  // (the last set has been read)
+    int any_bad = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) any_bad |= s_bad[w];
+    if constexpr (KS == 1) {
+        if (row >= u.rows) return;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                f32x4 acc = {O[dt][4 * b], O[dt][4 * b + 1], O[dt][4 * b + 2], O[dt][4 * b + 3]};
+                const int d0 = 32 * dt + 8 * b + 4 * h;
+                if (any_bad) acc = add_bad(acc, d0);
+                write(row, d0, acc, m, l);
+            }
+    } else {
+        // every stream leaves (m, l, O) in LDS; then wave (qg, ks) combines its share of the
+        // group's dims: slots of four consecutive dims of a column
+        constexpr int SL = DT * 4 / KS;  // slots per wave
+        static_assert(DT * 4 % KS == 0, "slots divide among the streams");
+        f32x4* part = reinterpret_cast<f32x4*>(&lds.kv[0][0][0]);
+        auto slot = [&](int k, int i4) { return part + ((k * QG + qg) * (DT * 4) + i4) * kWave + lane; };
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                *slot(ks, dt * 4 + b) = f32x4{O[dt][4 * b], O[dt][4 * b + 1], O[dt][4 * b + 2], O[dt][4 * b + 3]};
+        if (h == 0) {
+            s_ml[ks][qg][l32][0] = m;
+            s_ml[ks][qg][l32][1] = l;
+        }
+        __syncthreads();
+        float M = -FLT_MAX, lt = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) M = fmaxf(M, s_ml[k][qg][l32][0]);
+        f32x4 acc[SL];
+#pragma unroll
+        for (int i = 0; i < SL; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const float wk = fast_exp2(s_ml[k][qg][l32][0] - M);
+            lt = __builtin_fmaf(wk, s_ml[k][qg][l32][1], lt);
+#pragma unroll
+            for (int i = 0; i < SL; ++i) {
+                const f32x4 x = *slot(k, ks * SL + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][e] = __builtin_fmaf(wk, x[e], acc[i][e]);
+            }
+        }
+        if (row >= u.rows) return;
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            const int d0 = 8 * (ks * SL + i) + 4 * h;
+            if (any_bad) acc[i] = add_bad(acc[i], d0);
+            write(row, d0, acc[i], M, lt);
+        }
+    }
+}
+
+template <int D, int CT>
+__global__ __launch_bounds__(8 * kWave) void chunk_tile_kernel(ChunkParams p) {
+    __shared__ __attribute__((aligned(16))) TileLds<D> lds;
+    ChunkUnit u;
+    if (!chunk_unit(p, u) || u.kind != kKindTile) return;
+    if (u.rows <= 64) tile_unit<D, CT, 2>(p, u, lds);
+    else if (u.rows <= 128) tile_unit<D, CT, 4>(p, u, lds);
+    else if (u.rows <= 256) tile_unit<D, CT, 8>(p, u, lds);
+}
+
+}  // namespace
+}  // namespace kvc
