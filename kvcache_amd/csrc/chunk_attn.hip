@@ -117,7 +117,8 @@ int launch_chunks_d(const ChunkParams& p, int n_tiles, hipStream_t st) {
         if (matrix_path(D, p.block)) {
             if (n_tiles > 0) {  // the list's tiles come first
                 const dim3 tgrid((unsigned)((size_t)std::min(n_tiles, p.n_units - 1) * p.Hkv));
-                hipLaunchKernelGGL((chunk_tile_kernel<D, CT>), tgrid, dim3(8 * kWave), 0, st, p);
+                if (p.cap_log2 > 0.f) hipLaunchKernelGGL((chunk_tile_kernel<D, CT, true>), tgrid, dim3(8 * kWave), 0, st, p);
+                else hipLaunchKernelGGL((chunk_tile_kernel<D, CT, false>), tgrid, dim3(8 * kWave), 0, st, p);
                 const int rc = hip_check(hipGetLastError(), "chunk attention launch");
                 if (rc) return rc;
             }

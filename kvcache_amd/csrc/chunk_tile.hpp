@@ -87,7 +87,7 @@ struct TileLds {
     char kv[2][2][kSetKeys * D * 2];  // [half][K / V]
 };
 
-template <int D, int CT, int QG>
+template <int D, int CT, int QG, bool CAP>
 __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit& u, TileLds<D>& lds) {
     constexpr bool Q8 = CT != kCacheF16;
     constexpr int W = 8;
@@ -113,14 +113,20 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     const int bsh = __builtin_ctz((unsigned)p.block), bmask = p.block - 1;
     const char* kb = static_cast<const char*>(p.k);
     const char* vb = static_cast<const char*>(p.v);
-    const bool cap = p.cap_log2 > 0.f;
-    const float to_log2 = cap ? p.cap_in : p.scale_log2;
+    const float to_log2 = CAP ? p.cap_in : p.scale_log2;
 
-    // this wave's rows of set s; block ids one set per lane, 64 sets at a time
-    auto first_tok = [&](int s) { return j0 + s * kSetKeys + 16 * wave; };
+    // Sets [f0, f1) are seen whole by every row; they come first, then those before them (the
+    // window's edge) and after them (the causal one): the i-th set to come is set_at(i).
+    const int plast = u.pos0 + u.ntok - 1;
+    const int f0 = p.window > 0 ? min(nsets, max(0, plast - p.window + 1 - j0 + kSetKeys - 1) / kSetKeys) : 0;
+    const int f1 = max(f0, (min(u.pos0 + 1, j1) - j0) / kSetKeys);
+    const int nfull = f1 - f0;
+    auto set_at = [&](int i) { return i < nfull ? f0 + i : i - nfull < f0 ? i - nfull : i; };
+    // this wave's rows of the i-th set; block ids one set per lane, 64 sets at a time
+    auto first_tok = [&](int i) { return j0 + set_at(i) * kSetKeys + 16 * wave; };
     int ids = 0;
-    auto load_ids = [&](int s) {
-        ids = p.table[min(u.tab + (min(first_tok(s + lane), j1 - 1) >> bsh), p.table_len - 1)];
+    auto load_ids = [&](int i) {
+        ids = p.table[min(u.tab + (min(first_tok(i + lane), j1 - 1) >> bsh), p.table_len - 1)];
     };
     u32x4 rk[VL], rv[VL];
     f32x2 sc[VL];
@@ -196,7 +202,6 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     }
     const int wfirst = u.pos0 + min(32 * qg, u.rows - 1) / u.hn;      // positions of the wave's rows
     const int wlast = u.pos0 + min(32 * qg + 31, u.rows - 1) / u.hn;
-    const int plast = u.pos0 + u.ntok - 1;
 
     float ref = 0.f, l = 0.f;    // reference of p; sum of the lane's own keys
     float thr = -FLT_MAX;        // a relative score above it moves the reference (none met yet: any)
@@ -207,8 +212,8 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) O[dt][i] = 0.f;
-    const bool direct = Q8 && !cap;  // the accumulator is the relative score
-    if (direct) {
+    constexpr bool direct = Q8 && !CAP;  // the accumulator is the relative score
+    if constexpr (direct) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) C[i] = kBias;
     }
@@ -244,9 +249,9 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
                 const int c = 32 * n + 8 * (i >> 2) + (i & 3);
                 return !MASKED || (c <= lim && c > low);
             };
-            if (!direct) {
+            if constexpr (!direct) {
                 const float off = kBias - ref;
-                if (cap) {
+                if constexpr (CAP) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) S[i] = capped(Q8 ? S[i] : S[i] * to_log2, 1.f, p.cap_log2) + off;
                 } else {
@@ -267,7 +272,7 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
                 l *= corr;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) S[i] -= by;
-                if (direct) {
+                if constexpr (direct) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) C[i] = kBias - ref;
                 }
@@ -303,32 +308,24 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
         }
     };
 
-    // sets that every row sees whole: [f0, f1); before them the window's edge, after them the causal one
-    const int f0 = p.window > 0 ? min(nsets, max(0, plast - p.window + 1 - j0 + kSetKeys - 1) / kSetKeys) : 0;
-    const int f1 = max(f0, (min(u.pos0 + 1, j1) - j0) / kSetKeys);
-    auto whole = [&](int s) { return s >= f0 && s < f1; };
-    store(0, !whole(0));
+    store(0, nfull == 0);
     issue(1);
     // one set: the next one from its registers into the other half of the buffer, the one after
     // that into flight, then this one's arithmetic
-    auto set = [&](int s, auto masked_tag) {
+    auto set = [&](int i, auto masked_tag) {
         __syncthreads();
-        store((s + 1) & 1, decltype(masked_tag)::value || s + 1 >= f1);
-        if (((s + 2) & (kWave - 1)) == 0) load_ids(s + 2);
-        issue(s + 2);  // (sets past the end read nothing: zero-size descriptors)
-        const int t0 = j0 + s * kSetKeys + ks * KT;
+        store((i + 1) & 1, decltype(masked_tag)::value || i + 1 >= nfull);
+        if (((i + 2) & (kWave - 1)) == 0) load_ids(i + 2);
+        issue(i + 2);  // (sets past the last read nothing: zero-size descriptors)
+        const int t0 = j0 + set_at(i) * kSetKeys + ks * KT;
         if (!decltype(masked_tag)::value ||
             (32 * qg < u.rows && t0 <= wlast && t0 < j1 && (p.window <= 0 || t0 + KT > wfirst - p.window + 1)))
-            compute(s & 1, t0, masked_tag);
+            compute(i & 1, t0, masked_tag);
     };
     // (loops of their own: one loop with both forms copied O between them in every set)
-    int s = 0;
-    for (int end = f0;;) {
-        for (; s < end; ++s) set(s, std::true_type{});
-        if (end == nsets) break;
-        for (; s < f1; ++s) set(s, std::false_type{});
-        end = nsets;
-    }
+    int i = 0;
+    for (; i < nfull; ++i) set(i, std::false_type{});
+    for (; i < nsets; ++i) set(i, std::true_type{});
     l = sum_xor32(l);
     const float m = thr > -FLT_MAX ? ref : -FLT_MAX;
 
@@ -412,14 +409,14 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     }
 }
 
-template <int D, int CT>
+template <int D, int CT, bool CAP>
 __global__ __launch_bounds__(8 * kWave) void chunk_tile_kernel(ChunkParams p) {
     __shared__ __attribute__((aligned(16))) TileLds<D> lds;
     ChunkUnit u;
     if (!chunk_unit(p, u) || u.kind != kKindTile) return;
-    if (u.rows <= 64) tile_unit<D, CT, 2>(p, u, lds);
-    else if (u.rows <= 128) tile_unit<D, CT, 4>(p, u, lds);
-    else if (u.rows <= 256) tile_unit<D, CT, 8>(p, u, lds);
+    if (u.rows <= 64) tile_unit<D, CT, 2, CAP>(p, u, lds);
+    else if (u.rows <= 128) tile_unit<D, CT, 4, CAP>(p, u, lds);
+    else if (u.rows <= 256) tile_unit<D, CT, 8, CAP>(p, u, lds);
 }
 
 }  // namespace
