@@ -404,26 +404,29 @@ int kvc_read_kv(void* k, void* v, const void* k_pool, const void* v_pool, const 
  * [rows, Hq, D] fp16, the sequences' tokens one after the other; statistics are fp32.  A row
  * whose scores are all -Inf gets zeros; NaN and Inf in K or V reach the rows that see their key.
  *
+ * K and V values of up to 65504 in size (fp16's range) count as what they are, larger ones may
+ * count as Inf.
+ *
  * kvc_chunk_plan (host, once per step): cuts the batch into units and writes them into `work`
  *   (host memory of capacity * 16 ints; NULL: only counts).  capacity and *n_units are in
- *   entries of 16 ints, the list's header (entry 0) included; *n_tiles says how many units are
- *   tiles of many rows; *n_records is the partial rows of split key ranges.  host_tab_off
- *   (N + 1, NULL: tables packed in sequence order) locates each sequence's table in table_all.
- *   The caller copies the list to the device.
+ *   entries of 16 ints, the list's header (entry 0) included; *n_tiles of the units are tiles of
+ *   many rows; *n_records is the partial rows of split key ranges, *n_wide the keys that tiles
+ *   over an 8-bit cache hold as fp16 in the workspace.  host_tab_off (N + 1, NULL: tables packed
+ *   in sequence order) locates each sequence's table in table_all.  The caller copies the list
+ *   to the device.
  * kvc_paged_chunk_attn: runs it (same shape, kv_dtype and window; tuning knobs play no part).
- *   Every table read is bounded by table_len, every row by rows.  n_units, n_tiles and n_records
- *   may exceed the list's own counts (a captured graph replays lists of any smaller size that
- *   are copied to the same address; n_tiles > 0 then admits lists with tiles, and with
- *   n_tiles 0 a list that holds tiles leaves their rows unwritten).  workspace:
- *   kvc_chunk_workspace_size bytes, 16-byte aligned, any contents; NULL: library-owned (not
- *   under stream capture); launches that may overlap need workspaces of their own. */
+ *   Every table read is bounded by table_len, every row by rows.  n_tiles, n_units - n_tiles,
+ *   n_records and n_wide may exceed the list's own counts: a captured graph replays any list
+ *   within them that is copied to the same address.  workspace: kvc_chunk_workspace_size bytes
+ *   for the counts passed, 16-byte aligned, any contents; NULL: library-owned (not under stream
+ *   capture); launches that may overlap need workspaces of their own. */
 int kvc_chunk_plan(const int* host_q_lens, const int* host_kv_lens, const int* host_tab_off, int N, int Hq, int Hkv,
                    int D, int BLOCK, int kv_dtype, int window, int* work, int capacity, int* n_units, int* n_tiles,
-                   int* n_records);
-size_t kvc_chunk_workspace_size(int Hq, int Hkv, int D, int n_records);
+                   int* n_records, int* n_wide);
+size_t kvc_chunk_workspace_size(int Hq, int Hkv, int D, int n_records, int n_wide);
 int kvc_paged_chunk_attn(const void* q, void* out, const void* k_pool, const void* v_pool, const float* kv_scales,
                          const int* table_all, int table_len, const int* work, int n_units, int n_tiles, int n_records,
-                         int rows, int Hq, int Hkv, int D, int BLOCK, float scale, float softcap, int window,
+                         int n_wide, int rows, int Hq, int Hkv, int D, int BLOCK, float scale, float softcap, int window,
                          int kv_dtype, void* workspace, size_t workspace_bytes, kvc_stream_t stream);
 
 /* ---- decoder-step operations around the attention path (a Qwen2-shaped layer) ----

@@ -150,10 +150,10 @@ _SIGS = {
         i32, [vp, vp, vp, vp, vp, C.c_longlong, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, i32, i32, vp]),
     "kvc_write_kv_q8": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
     "kvc_read_kv": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
-    "kvc_chunk_plan": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, i32, ip, ip, ip]),
-    "kvc_chunk_workspace_size": (sz, [i32, i32, i32, i32]),
+    "kvc_chunk_plan": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, i32, ip, ip, ip, ip]),
+    "kvc_chunk_workspace_size": (sz, [i32, i32, i32, i32, i32]),
     "kvc_paged_chunk_attn": (
-        i32, [vp] * 6 + [i32, vp] + [i32] * 8 + [f32, f32, i32, i32, vp, sz, vp]),
+        i32, [vp] * 6 + [i32, vp] + [i32] * 9 + [f32, f32, i32, i32, vp, sz, vp]),
     "kvc_embed_gather": (i32, [vp, vp, vp, i32, i32, i32, vp]),
     "kvc_rmsnorm": (i32, [vp, vp, vp, i32, i32, f32, vp]),
     "kvc_add_bias": (i32, [vp, vp, i32, i32, vp]),

@@ -13,14 +13,17 @@ namespace kvc {
 
 constexpr int kChunkInts = 16;
 enum ChunkHeader { kHdrUnits = 0, kHdrTiles = 1, kHdrRecords = 2 };
+// kFWide..kFWide1 (tiles over an 8-bit cache): the workspace row of key kFWideKey of the sequence,
+// and the keys that this unit widens into it
 enum ChunkField { kFKind = 0, kFRow = 1, kFTok = 2, kFPos = 3, kFHead = 4, kFHeads = 5, kFJ0 = 6, kFJ1 = 7, kFChunk = 8,
-                  kFChunks = 9, kFRec = 10, kFTab = 11 };
+                  kFChunks = 9, kFRec = 10, kFTab = 11, kFWide = 12, kFWideKey = 13, kFWide0 = 14, kFWide1 = 15 };
 enum ChunkKind { kKindRows = 0, kKindTile = 1 };
 
 struct ChunkParams {
     const int* work;
     int n_units;            // entries of the list the grid covers, the header included
     int n_records;          // partial rows per KV head that the workspace holds
+    int n_wide;             // ... and widened keys
     int rows, Hq, Hkv, group, block;
     int table_len, window;
     float scale_log2;       // softmax scale * log2(e)
@@ -34,19 +37,23 @@ struct ChunkParams {
     const int* table;
     float* part_acc;        // [Hkv][n_records][D]
     float* part_ml;         // [Hkv][n_records][2]
+    _Float16* wide_k;       // [Hkv][n_wide][D]
+    _Float16* wide_v;
 };
 
 namespace {
 
 struct ChunkUnit {
     int kind, row0, ntok, pos0, h0, hn, j0, j1, c, nc, rec0, tab;
+    int wide, wkey, w0, w1;
     int hk;
     int rows;   // ntok * hn
 };
 
-// The workgroup's unit; false past the list's end and for entries that do not fit the launch.
-__device__ __forceinline__ bool chunk_unit(const ChunkParams& p, ChunkUnit& u) {
-    const int i = (int)(blockIdx.x / (unsigned)p.Hkv) + 1;
+// The workgroup's unit, the list's entry 1 + skip + blockIdx.x / Hkv; false past the list's end and
+// for entries that do not fit the launch.
+__device__ __forceinline__ bool chunk_unit(const ChunkParams& p, ChunkUnit& u, int skip) {
+    const int i = (int)(blockIdx.x / (unsigned)p.Hkv) + 1 + skip;
     if (i >= min(p.work[kHdrUnits], p.n_units)) return false;
     const int* e = p.work + (size_t)i * kChunkInts;
     u.kind = e[kFKind];
@@ -61,11 +68,18 @@ __device__ __forceinline__ bool chunk_unit(const ChunkParams& p, ChunkUnit& u) {
     u.nc = e[kFChunks];
     u.rec0 = e[kFRec];
     u.tab = e[kFTab];
+    u.wide = e[kFWide];
+    u.wkey = e[kFWideKey];
+    u.w0 = e[kFWide0];
+    u.w1 = e[kFWide1];
     u.hk = (int)(blockIdx.x % (unsigned)p.Hkv);
     u.rows = u.ntok * u.hn;
     return u.row0 >= 0 && u.ntok > 0 && u.row0 <= p.rows - u.ntok && u.h0 >= 0 && u.hn > 0 && u.h0 <= p.group - u.hn &&
            u.j0 >= 0 && u.pos0 >= 0 && u.tab >= 0 && u.c >= 0 && u.c < u.nc &&
-           (u.nc == 1 || (u.rec0 >= 0 && (long long)u.rec0 + (long long)u.nc * u.rows <= p.n_records));
+           (u.nc == 1 || (u.rec0 >= 0 && (long long)u.rec0 + (long long)u.nc * u.rows <= p.n_records)) &&
+           (u.kind != kKindTile || p.n_wide == 0 ||
+            (u.wide >= 0 && u.wkey >= 0 && u.wkey <= u.j0 && u.w0 >= u.wkey &&
+             (long long)u.wide + (max(u.j1, u.w1) - u.wkey) <= p.n_wide));
 }
 
 // Element offset of row r of the unit in q and out.
@@ -89,7 +103,7 @@ __global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkParams p) {
     constexpr int NJ = (D + kWave - 1) / kWave;
     __shared__ float s_q[4][D];
     ChunkUnit u;
-    if (!chunk_unit(p, u)) return;
+    if (!chunk_unit(p, u, 0)) return;
     const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6);
     for (int r = wave; r < u.rows; r += 4) {
         const size_t qo = chunk_row(p, u, r, D);
@@ -564,7 +578,7 @@ template <int D, int CT>
 __global__ __launch_bounds__((StreamShape<D, CT>::W * kWave), (D == 64 ? 4 : 2)) void chunk_stream_kernel(ChunkParams p) {
     __shared__ __attribute__((aligned(16))) char lds[StreamShape<D, CT>::kBytes];
     ChunkUnit u;
-    if (!chunk_unit(p, u) || u.kind != kKindRows) return;
+    if (!chunk_unit(p, u, max(p.work[kHdrTiles], 0)) || u.kind != kKindRows) return;
     if (u.rows <= 16) stream_unit<D, CT, 1>(p, u, lds);
 }
 
@@ -577,7 +591,7 @@ __global__ __launch_bounds__(256) void merge_chunks_kernel(ChunkParams p) {
     __shared__ f32x4 s_acc[SLOTS][TD];
     __shared__ float s_ml[SLOTS][2];
     ChunkUnit u;
-    if (!chunk_unit(p, u) || u.nc == 1) return;
+    if (!chunk_unit(p, u, 0) || u.nc == 1) return;
     const int slot = threadIdx.x / TD, d = threadIdx.x % TD * 4;
     const int n = min(SLOTS, u.nc);
     for (int r = u.c; r < u.rows; r += u.nc) {

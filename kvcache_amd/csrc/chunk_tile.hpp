@@ -1,17 +1,21 @@
 // chunk_tile.hpp -- chunk attention of many rows on the matrix cores (head_dim 64 / 128).
 //
-// A workgroup of 8 waves takes 32 QG rows (token, head) of one KV head, QG groups of 32 rows
-// times KS = 8 / QG key streams.  Keys come in sets of 128, stream ks of a set taking its
-// 128 / KS keys.  Wave w brings rows 16 w .. + 15 of a set (one block id, whole rows, rows past
-// the end read as zero through the descriptor) into registers while the set before is computed,
-// then, as fp16, into the other half of the LDS buffer; one barrier per set.
+// 8-bit caches: widen_kernel first turns the keys that tiles see into fp16 rows in the workspace,
+// K times its scale and the factor to log2 units, V times its scale, each product rounded once
+// (what an fp16 cache would hold; values beyond fp16's range, 65504, become Inf).  Every tile of a
+// sequence reads all of its keys, so widening them in the tiles costs the more the more tiles
+// there are: 2000 tokens of 32 heads behind 6000, D 128, were 316 us with it in the tiles (about as
+// many vector instructions as the softmax has).
 //
-//   8-bit rows become fp16 on their way into LDS, once for all rows of the workgroup: K times
-//     its scale and the factor to log2 units, V times its scale, each product rounded once (what
-//     an fp16 cache would hold; values beyond fp16's range, 65504, become Inf).
+// tile_unit: a workgroup of 8 waves takes 32 QG rows (token, head) of one KV head, QG groups of 32
+// rows times KS = 8 / QG key streams.  Keys come in sets of 128, stream ks of a set taking its 128 /
+// KS keys.  Wave w brings rows 16 w .. + 15 of a set (one block id, whole rows, rows past the end
+// read as zero through the descriptor) into registers while the set before is computed, then into
+// the other half of the LDS buffer; one barrier per set.
+//
 //   S^T[key][row] = K Q^T with v_mfma_f32_32x32x16_f16: a lane holds 16 scores of ONE row
-//     (column l % 32), so a row's maximum needs one exchange with lane l ^ 32.  8-bit caches
-//     start the accumulator at kBias - reference, so the products' sum is the exponent itself.
+//     (column l % 32), so a row's maximum needs one exchange with lane l ^ 32.  Widened keys:
+//     the accumulator starts at kBias - reference, so the products' sum is the exponent itself.
 //   softmax: p = 2^(s - reference + kBias), fp32, then fp16.  The reference lags: it moves to the
 //     row's maximum when a score passes it by more than 2^kLag (and at a row's first key), so p
 //     is at most 2^15, fp16 keeps all its bits down to 2^-21 of the largest, and O is rescaled a
@@ -19,6 +23,7 @@
 //     probabilities (two a v_dot2), the ones O is made of.
 //   O^T[dim][row] += V^T P^T: the lane's own probabilities are the operand up to the order of
 //     keys, and V^T is read back in that order with the transposing LDS read.
+// A wave's scores of the next 32 keys are computed while the exponentials of these are taken.
 //
 // LDS: K rows as 16-byte chunks XOR-permuted by the row, V rows as 32-byte segments permuted by
 // the row, so that neither operand read meets a bank twice.
@@ -59,25 +64,33 @@ __device__ __forceinline__ void scaled_f16(u32x4 c, float s, u32x4 (&out)[2]) {
 
 __device__ __forceinline__ float row_factor(float s) { return __uint_as_float(__float_as_uint(s) & 0xFFFFFFF0u); }
 
-// add_seen_nonfinite (chunk_attn.hpp) of the elements as tile_unit stages them.
+// A tile's share of its sequence's keys, as fp16 rows of the workspace.
+constexpr int kWidenBlocks = 16;  // workgroups per tile and KV head
 template <int D, int CT>
-__device__ __forceinline__ f32x4 add_seen_nonfinite_q8(const ChunkParams& p, const ChunkUnit& u, f32x4 acc, int pos, int d0) {
-    const int bsh = __builtin_ctz((unsigned)p.block);
-    const int first = max(u.j0, p.window > 0 ? pos - p.window + 1 : 0), last = min(u.j1 - 1, pos);
-    for (int j = first; j <= last; ++j) {
-        const int id = p.table[min(u.tab + (j >> bsh), p.table_len - 1)];
-        const size_t row = (((size_t)(unsigned)(id * p.Hkv + u.hk)) << bsh) + (j & (p.block - 1));
-        f16x2 a, b;
-        codes_to_f16<CT>(*reinterpret_cast<const unsigned*>(static_cast<const char*>(p.v) + row * D + d0), a, b);
-        const float s = row_factor(p.scales[row * 2 + 1]);
-        const f16x4 v = {(_Float16)((float)a[0] * s), (_Float16)((float)a[1] * s), (_Float16)((float)b[0] * s),
-                         (_Float16)((float)b[1] * s)};
-        const u16x4 bits = __builtin_bit_cast(u16x4, v);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (nonfinite(bits[r])) acc[r] += (float)v[r];
+__global__ __launch_bounds__(256) void widen_kernel(ChunkParams p) {
+    constexpr int LPR = D / 16, RPB = 256 / LPR;
+    ChunkUnit u;
+    if (!chunk_unit(p, u, 0) || u.kind != kKindTile) return;
+    const int n = u.w1 - u.w0, per = (n + kWidenBlocks - 1) / kWidenBlocks;
+    const int k0 = u.w0 + blockIdx.y * per, k1 = min(k0 + per, u.w1);
+    const int l = threadIdx.x % LPR;
+    const float kf = p.cap_log2 > 0.f ? p.cap_in : p.scale_log2;
+    for (int k = k0 + threadIdx.x / LPR; k < k1; k += RPB) {
+        const int b = k / p.block;
+        const int id = p.table[min(u.tab + b, p.table_len - 1)];
+        const size_t row = ((size_t)(unsigned)(id * p.Hkv + u.hk)) * p.block + (k - b * p.block);
+        const size_t to = ((size_t)u.hk * p.n_wide + u.wide + (k - u.wkey)) * D + 16 * l;
+        const f32x2 s = *reinterpret_cast<const f32x2*>(p.scales + row * 2);
+        const u32x4 ck = *reinterpret_cast<const u32x4*>(static_cast<const char*>(p.k) + row * D + 16 * l);
+        const u32x4 cv = *reinterpret_cast<const u32x4*>(static_cast<const char*>(p.v) + row * D + 16 * l);
+        u32x4 x[2];
+        scaled_f16<CT>(ck, row_factor(s[0] * kf), x);
+        reinterpret_cast<u32x4*>(p.wide_k + to)[0] = x[0];
+        reinterpret_cast<u32x4*>(p.wide_k + to)[1] = x[1];
+        scaled_f16<CT>(cv, row_factor(s[1]), x);
+        reinterpret_cast<u32x4*>(p.wide_v + to)[0] = x[0];
+        reinterpret_cast<u32x4*>(p.wide_v + to)[1] = x[1];
     }
-    return acc;
 }
 
 constexpr int kSetKeys = 128;  // keys of an LDS set: 16 rows for each of 8 waves
@@ -87,19 +100,19 @@ struct TileLds {
     char kv[2][2][kSetKeys * D * 2];  // [half][K / V]
 };
 
-template <int D, int CT, int QG, bool CAP>
+// WIDE: keys from the workspace (widen_kernel), else from the pages of an fp16 cache.
+template <int D, bool WIDE, int QG, bool CAP>
 __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit& u, TileLds<D>& lds) {
-    constexpr bool Q8 = CT != kCacheF16;
     constexpr int W = 8;
-    constexpr int SRC = D * kCodeBytes<CT>;  // bytes of a cached row
-    constexpr int ROW = D * 2;               // ... of a row in LDS
+    constexpr int ROW = D * 2;               // bytes of a row
     constexpr int KS = W / QG;               // key streams
     constexpr int KT = kSetKeys / KS;        // keys per stream and set
     constexpr int NS = KT / 32;              // 32-key subtiles
     constexpr int KD = D / 16;               // MFMA k steps over the head dimension
     constexpr int DT = D / 32;               // 32-dim output tiles
-    constexpr int VL = 16 * SRC / 1024;      // wave loads per 16 rows
+    constexpr int VL = 16 * ROW / 1024;      // wave loads per 16 rows
     constexpr int kSetBytes = kSetKeys * ROW;
+    constexpr bool direct = WIDE && !CAP;    // the accumulator is the relative score
     static_assert(KS == 1 || KS * QG * 32 * D * 4 <= 2 * 2 * kSetBytes, "partials fit the tile buffers");
     __shared__ float s_ml[KS][QG][32][2];
     __shared__ int s_bad[W];
@@ -111,9 +124,8 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     const int j0 = u.j0, j1 = u.j1;
     const int nsets = (j1 - j0 + kSetKeys - 1) / kSetKeys;
     const int bsh = __builtin_ctz((unsigned)p.block), bmask = p.block - 1;
-    const char* kb = static_cast<const char*>(p.k);
-    const char* vb = static_cast<const char*>(p.v);
-    const float to_log2 = CAP ? p.cap_in : p.scale_log2;
+    const char* kb = WIDE ? reinterpret_cast<const char*>(p.wide_k) : static_cast<const char*>(p.k);
+    const char* vb = WIDE ? reinterpret_cast<const char*>(p.wide_v) : static_cast<const char*>(p.v);
 
     // Sets [f0, f1) are seen whole by every row; they come first, then those before them (the
     // window's edge) and after them (the causal one): the i-th set to come is set_at(i).
@@ -126,30 +138,25 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     auto first_tok = [&](int i) { return j0 + set_at(i) * kSetKeys + 16 * wave; };
     int ids = 0;
     auto load_ids = [&](int i) {
-        ids = p.table[min(u.tab + (min(first_tok(i + lane), j1 - 1) >> bsh), p.table_len - 1)];
+        if constexpr (!WIDE) ids = p.table[min(u.tab + (min(first_tok(i + lane), j1 - 1) >> bsh), p.table_len - 1)];
+    };
+    auto row_of = [&](int t, int id) -> size_t {
+        if constexpr (WIDE) return (size_t)u.hk * p.n_wide + u.wide + (t - u.wkey);
+        else return (((size_t)(unsigned)(id * p.Hkv + u.hk)) << bsh) + (t & bmask);
     };
     u32x4 rk[VL], rv[VL];
-    f32x2 sc[VL];
-    int i_rows = 0;
-    size_t i_row = 0;
-    auto issue = [&](int s) {
-        const int t = first_tok(s);
-        const int id = __builtin_amdgcn_readlane(ids, s & (kWave - 1));
+    auto issue = [&](int i) {
+        const int t = first_tok(i);
+        const int id = WIDE ? 0 : __builtin_amdgcn_readlane(ids, i & (kWave - 1));
         int rows = max(j1 - t, 0);
         asm("" : "+s"(rows));
-        i_rows = min(rows, 16);
-        i_row = (((size_t)(unsigned)(id * p.Hkv + u.hk)) << bsh) + (t & bmask);
-        const __amdgpu_buffer_rsrc_t kr = tile_rsrc(kb + i_row * SRC, i_rows * SRC), vr = tile_rsrc(vb + i_row * SRC, i_rows * SRC);
+        const int bytes = min(rows, 16) * ROW;
+        const size_t off = row_of(rows > 0 ? t : j0, id) * ROW;
+        const __amdgpu_buffer_rsrc_t kr = tile_rsrc(kb + off, bytes), vr = tile_rsrc(vb + off, bytes);
 #pragma unroll
-        for (int i = 0; i < VL; ++i) rk[i] = buffer_load16(kr, i * 1024 + lane * 16);
+        for (int n = 0; n < VL; ++n) rk[n] = buffer_load16(kr, n * 1024 + lane * 16);
 #pragma unroll
-        for (int i = 0; i < VL; ++i) rv[i] = buffer_load16(vr, i * 1024 + lane * 16);
-        if constexpr (Q8) {  // (rows past the end read as scale 0)
-            const __amdgpu_buffer_rsrc_t sr = tile_rsrc(p.scales + i_row * 2, i_rows * 8);
-#pragma unroll
-            for (int i = 0; i < VL; ++i)
-                sc[i] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(sr, (i * 1024 + lane * 16) / SRC * 8, 0, 0));
-        }
+        for (int n = 0; n < VL; ++n) rv[n] = buffer_load16(vr, n * 1024 + lane * 16);
     };
     auto kchunk = [](int r, int ch) { return ch ^ (r & 7); };
     auto vseg = [](int r, int seg) { return seg ^ (D == 64 ? (r >> 1) & 3 : r & 7); };
@@ -157,35 +164,16 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     auto store = [&](int half, bool edge) {
         char* kd = lds.kv[half][0];
         char* vd = lds.kv[half][1];
-        if constexpr (Q8) {
+        if (edge && any_nonfinite(rv)) {
+            clear_nonfinite(rv);
+            bad = true;
+        }
 #pragma unroll
-            for (int i = 0; i < VL; ++i) {
-                const int off = i * 1024 + lane * 16;
-                const int r = 16 * wave + off / SRC, c = off % SRC / 8;  // first of two 16-byte chunks
-                u32x4 x[2];
-                scaled_f16<CT>(rk[i], row_factor(sc[i][0] * to_log2), x);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) *reinterpret_cast<u32x4*>(kd + r * ROW + kchunk(r, c + e) * 16) = x[e];
-                scaled_f16<CT>(rv[i], row_factor(sc[i][1]), x);
-                if (edge && any_nonfinite(x)) {
-                    clear_nonfinite(x);
-                    bad = true;
-                }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) *reinterpret_cast<u32x4*>(vd + r * ROW + vseg(r, c >> 1) * 32 + e * 16) = x[e];
-            }
-        } else {
-            if (edge && any_nonfinite(rv)) {
-                clear_nonfinite(rv);
-                bad = true;
-            }
-#pragma unroll
-            for (int i = 0; i < VL; ++i) {
-                const int off = i * 1024 + lane * 16;
-                const int r = 16 * wave + off / ROW, cb = off % ROW;
-                *reinterpret_cast<u32x4*>(kd + r * ROW + kchunk(r, cb >> 4) * 16) = rk[i];
-                *reinterpret_cast<u32x4*>(vd + r * ROW + vseg(r, cb >> 5) * 32 + (cb & 31)) = rv[i];
-            }
+        for (int n = 0; n < VL; ++n) {
+            const int off = n * 1024 + lane * 16;
+            const int r = 16 * wave + off / ROW, cb = off % ROW;
+            *reinterpret_cast<u32x4*>(kd + r * ROW + kchunk(r, cb >> 4) * 16) = rk[n];
+            *reinterpret_cast<u32x4*>(vd + r * ROW + vseg(r, cb >> 5) * 32 + (cb & 31)) = rv[n];
         }
     };
 
@@ -207,16 +195,11 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     float thr = -FLT_MAX;        // a relative score above it moves the reference (none met yet: any)
     f32x16 O[DT], C;             // C: what the score accumulator starts from
 #pragma unroll
-    for (int i = 0; i < 16; ++i) C[i] = 0.f;
+    for (int i = 0; i < 16; ++i) C[i] = direct ? kBias : 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) O[dt][i] = 0.f;
-    constexpr bool direct = Q8 && !CAP;  // the accumulator is the relative score
-    if constexpr (direct) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) C[i] = kBias;
-    }
 
     int ka[4], va[DT];
 #pragma unroll
@@ -242,26 +225,28 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
         // S[i] is key t0 + 32 n + 8 (i / 4) + 4 h + i % 4, seen when low < 32 n + 8 (i / 4) + i % 4 <= lim
         const int lim = min(pos, j1 - 1) - t0 - 4 * h;
         const int low = (p.window > 0 ? pos - p.window : -1) - t0 - 4 * h;
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            f32x16 S = scores(n);
-            auto seen = [&](int i) {
-                const int c = 32 * n + 8 * (i >> 2) + (i & 3);
-                return !MASKED || (c <= lim && c > low);
-            };
+        // relative scores, those of unseen keys -Inf; the reference moves where one is too far above it
+        auto settle = [&](f32x16& S, int n) {
             if constexpr (!direct) {
                 const float off = kBias - ref;
                 if constexpr (CAP) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) S[i] = capped(Q8 ? S[i] : S[i] * to_log2, 1.f, p.cap_log2) + off;
+                    for (int i = 0; i < 16; ++i) S[i] = capped(S[i], WIDE ? 1.f : p.cap_in, p.cap_log2) + off;
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) S[i] = __builtin_fmaf(S[i], to_log2, off);
+                    for (int i = 0; i < 16; ++i) S[i] = __builtin_fmaf(S[i], p.scale_log2, off);
+                }
+            }
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int c = 32 * n + 8 * (i >> 2) + (i & 3);
+                    S[i] = c <= lim && c > low ? S[i] : -__builtin_inff();
                 }
             }
             float mx = -FLT_MAX;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = seen(i) ? fmaxf(mx, S[i]) : mx;
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[i]);
             if (__any(mx > thr)) {
                 mx = max_xor32(mx);
                 const bool move = mx > thr;
@@ -281,29 +266,39 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
 #pragma unroll
                     for (int i = 0; i < 16; ++i) O[dt][i] *= corr;
             }
+        };
+        f32x16 S = scores(0);
+        settle(S, 0);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            f32x16 next = C;
+            if (n + 1 < NS) next = scores(n + 1);
+            f16x8v pb[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                f16x8v pb;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float e = fast_exp2(S[8 * t + j]);
-                    pb[j] = (_Float16)(seen(8 * t + j) ? e : 0.f);
-                }
+                for (int j = 0; j < 8; ++j) pb[t][j] = (_Float16)fast_exp2(S[8 * t + j]);
                 const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
-                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb, pb, 0, 1), one, l, false);
-                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb, pb, 2, 3), one, l, false);
-                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb, pb, 4, 5), one, l, false);
-                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb, pb, 6, 7), one, l, false);
-                // V^T operand: k slots (h, j) are keys 32 n + 16 t + 8 (j / 4) + 4 h + j % 4, of dim
-                // 32 dt + l % 32; two transposing reads of four keys each (16 lanes address four
-                // rows of 16 dims: lane i row i / 4, dims 4 (i % 4) .. + 3)
+                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 0, 1), one, l, false);
+                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 2, 3), one, l, false);
+                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 4, 5), one, l, false);
+                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 6, 7), one, l, false);
+            }
+            // V^T operand: k slots (h, j) are keys 32 n + 16 t + 8 (j / 4) + 4 h + j % 4, of dim 32 dt
+            // + l % 32; two transposing reads of four keys each (16 lanes address four rows of 16
+            // dims: lane i row i / 4, dims 4 (i % 4) .. + 3)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
                     const char* vt = buf + va[dt] + (32 * n + 16 * t) * ROW;
                     const s16x4v lo = ds_read_tr16(vt), hi = ds_read_tr16(vt + 8 * ROW);
                     const f16x8v a = __builtin_bit_cast(f16x8v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                    O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pb, O[dt], 0, 0, 0);
+                    O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pb[t], O[dt], 0, 0, 0);
                 }
+            if (n + 1 < NS) {
+                settle(next, n + 1);
+                S = next;
             }
         }
     };
@@ -315,7 +310,7 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     auto set = [&](int i, auto masked_tag) {
         __syncthreads();
         store((i + 1) & 1, decltype(masked_tag)::value || i + 1 >= nfull);
-        if (((i + 2) & (kWave - 1)) == 0) load_ids(i + 2);
+        if (!WIDE && ((i + 2) & (kWave - 1)) == 0) load_ids(i + 2);
         issue(i + 2);  // (sets past the last read nothing: zero-size descriptors)
         const int t0 = j0 + set_at(i) * kSetKeys + ks * KT;
         if (!decltype(masked_tag)::value ||
@@ -345,9 +340,17 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
             }
         }
     };
+    // Inf and NaN of V (as staged) of the keys that this lane's row sees, as add_seen_nonfinite
     auto add_bad = [&](f32x4 acc, int d0) {
-        if constexpr (Q8) return add_seen_nonfinite_q8<D, CT>(p, u, acc, pos, d0);
-        else return add_seen_nonfinite<D>(p, u, acc, pos, d0);
+        if constexpr (!WIDE) return add_seen_nonfinite<D>(p, u, acc, pos, d0);
+        for (int j = max(j0, p.window > 0 ? pos - p.window + 1 : 0); j <= min(j1 - 1, pos); ++j) {
+            const f16x4 v = *reinterpret_cast<const f16x4*>(p.wide_v + row_of(j, 0) * D + d0);
+            const u16x4 bits = __builtin_bit_cast(u16x4, v);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (nonfinite(bits[r])) acc[r] += (float)v[r];
+        }
+        return acc;
     };
     if (lane == 0) s_bad[wave] = bad;
     __syncthreads();  // (the last set has been read)
@@ -409,14 +412,14 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     }
 }
 
-template <int D, int CT, bool CAP>
+template <int D, bool WIDE, bool CAP>
 __global__ __launch_bounds__(8 * kWave) void chunk_tile_kernel(ChunkParams p) {
     __shared__ __attribute__((aligned(16))) TileLds<D> lds;
     ChunkUnit u;
-    if (!chunk_unit(p, u) || u.kind != kKindTile) return;
-    if (u.rows <= 64) tile_unit<D, CT, 2, CAP>(p, u, lds);
-    else if (u.rows <= 128) tile_unit<D, CT, 4, CAP>(p, u, lds);
-    else if (u.rows <= 256) tile_unit<D, CT, 8, CAP>(p, u, lds);
+    if (!chunk_unit(p, u, 0) || u.kind != kKindTile) return;
+    if (u.rows <= 64) tile_unit<D, WIDE, 2, CAP>(p, u, lds);
+    else if (u.rows <= 128) tile_unit<D, WIDE, 4, CAP>(p, u, lds);
+    else if (u.rows <= 256) tile_unit<D, WIDE, 8, CAP>(p, u, lds);
 }
 
 }  // namespace

@@ -218,7 +218,7 @@ def read_kv(k, v, k_pool, v_pool, kv_scales, slot_map, rows, Hkv, D, BLOCK, *, d
 
 def chunk_plan(q_lens, kv_lens, Hq, Hkv, D, BLOCK, *, tab_off=None, kv_dtype=KVC_I8, window=0):
     """Host-side plan of paged_chunk_attn (kvc_chunk_plan): returns (work [n_units, 16] int32,
-    n_units, n_tiles, n_records)."""
+    n_units, n_tiles, ws_rows), ws_rows the workspace's rows: (n_records, n_wide)."""
     import ctypes as C
 
     import numpy as np
@@ -228,30 +228,30 @@ def chunk_plan(q_lens, kv_lens, Hq, Hkv, D, BLOCK, *, tab_off=None, kv_dtype=KVC
     if q.shape != t.shape or q.ndim != 1 or (toff is not None and toff.shape != (len(q) + 1,)):
         raise KvcError(KVC_ERR_ARG, "q_lens and kv_lens hold one length per sequence, tab_off one entry more")
     tp = None if toff is None else toff.ctypes.data
-    nu, nt, nr = C.c_int(0), C.c_int(0), C.c_int(0)
+    nu, nt, nr, nw = (C.c_int(0) for _ in range(4))
     L = lib()
 
     def plan(work, cap):
         check(L.kvc_chunk_plan(q.ctypes.data, t.ctypes.data, tp, len(q), Hq, Hkv, D, BLOCK, kv_dtype, window, work, cap,
-                               C.byref(nu), C.byref(nt), C.byref(nr)))
+                               C.byref(nu), C.byref(nt), C.byref(nr), C.byref(nw)))
 
     plan(None, 0)
     work = np.zeros((nu.value, 16), dtype=np.int32)
     plan(work.ctypes.data, nu.value)
-    return work, nu.value, nt.value, nr.value
+    return work, nu.value, nt.value, (nr.value, nw.value)
 
 
-def chunk_workspace_size(Hq, Hkv, D, n_records) -> int:
-    return int(lib().kvc_chunk_workspace_size(Hq, Hkv, D, n_records))
+def chunk_workspace_size(Hq, Hkv, D, ws_rows) -> int:
+    return int(lib().kvc_chunk_workspace_size(Hq, Hkv, D, *ws_rows))
 
 
-def paged_chunk_attn(q, out, k_pool, v_pool, kv_scales, table_all, table_len, work_dev, n_units, n_tiles, n_records,
+def paged_chunk_attn(q, out, k_pool, v_pool, kv_scales, table_all, table_len, work_dev, n_units, n_tiles, ws_rows,
                      rows, Hq, Hkv, D, BLOCK, scale, *, kv_dtype=KVC_I8, softcap=0.0, window=0, workspace=None,
                      stream=None):
     """Attention of a ragged batch of chunks over a paged cache, on a plan of chunk_plan."""
     ws, wsb = _ws(workspace)
     check(lib().kvc_paged_chunk_attn(_p(q), _p(out), _p(k_pool), _p(v_pool), _p(kv_scales), _p(table_all),
-                                     int(table_len), _p(work_dev), n_units, n_tiles, n_records, rows, Hq, Hkv, D,
+                                     int(table_len), _p(work_dev), n_units, n_tiles, *ws_rows, rows, Hq, Hkv, D,
                                      BLOCK, scale, softcap, window, kv_dtype, ws, wsb, stream))
 
 

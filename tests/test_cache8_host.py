@@ -63,17 +63,17 @@ def test_write_and_read_refuse(f):
 
 def attn(**kw):
     a = dict(q=P, out=P, k_pool=P, v_pool=P, kv_scales=P, table_all=P, table_len=9, work_dev=P, n_units=3, n_tiles=0,
-             n_records=0, rows=4, Hq=8, Hkv=2, D=64, BLOCK=16, scale=0.125)
+             ws_rows=(0, 0), rows=4, Hq=8, Hkv=2, D=64, BLOCK=16, scale=0.125)
     a.update(kw)
     return ops.paged_chunk_attn(**a)
 
 
 @pytest.mark.parametrize("kw", [dict(Hq=9), dict(Hkv=0), dict(BLOCK=0), dict(window=-1), dict(kv_dtype=5), dict(rows=-1),
-                                dict(n_units=-1), dict(n_tiles=-1), dict(n_records=-1), dict(scale=np.nan),
+                                dict(n_units=-1), dict(n_tiles=-1), dict(ws_rows=(-1, 0)), dict(ws_rows=(0, -1)), dict(n_tiles=1), dict(scale=np.nan),
                                 dict(softcap=-1.0), dict(softcap=np.inf), dict(q=None), dict(out=P + 2),
                                 dict(k_pool=None), dict(v_pool=P + 8), dict(kv_scales=None), dict(kv_scales=P + 4),
                                 dict(table_all=None), dict(table_len=0), dict(work_dev=None),
-                                dict(n_records=9, workspace=(P + 4, 1 << 20))])
+                                dict(ws_rows=(9, 0), workspace=(P + 4, 1 << 20))])
 def test_chunk_attention_refuses(kw):
     refused(N.KVC_ERR_ARG, attn, **kw)
 
@@ -82,9 +82,9 @@ def test_chunk_attention_unsupported_and_workspace():
     refused(N.KVC_ERR_UNSUPPORTED, attn, D=80)
     refused(N.KVC_ERR_UNSUPPORTED, attn, kv_dtype=N.KVC_F32)
     refused(N.KVC_ERR_UNSUPPORTED, attn, n_units=1 << 30, Hkv=8)
-    need = ops.chunk_workspace_size(8, 2, 64, 100)
-    assert need >= 2 * 100 * (64 + 2) * 4 and ops.chunk_workspace_size(8, 2, 64, 0) == 0
-    refused(N.KVC_ERR_WORKSPACE, attn, n_records=100, workspace=(P, need - 1))
+    need = ops.chunk_workspace_size(8, 2, 64, (100, 50))
+    assert need >= 2 * 100 * (64 + 2) * 4 + 2 * 50 * 2 * 64 * 2 and ops.chunk_workspace_size(8, 2, 64, (0, 0)) == 0
+    refused(N.KVC_ERR_WORKSPACE, attn, ws_rows=(100, 50), workspace=(P, need - 1))
 
 
 def test_nothing_to_do_is_no_call():
@@ -106,13 +106,13 @@ def test_plan_refuses():
     refused(N.KVC_ERR_UNSUPPORTED, ops.chunk_plan, [0, 0], [2 ** 31 - 1] * 2, 8, 2, 64, 1)
     L = N.lib()
     import ctypes as C
-    n = [C.c_int(0) for _ in range(3)]
+    n = [C.c_int(0) for _ in range(4)]
     one = np.ones(1, np.int32)
     assert L.kvc_chunk_plan(one.ctypes.data, one.ctypes.data, None, 1, 8, 2, 64, 16, N.KVC_I8, 0, one.ctypes.data, 1,
                             *map(C.byref, n)) == N.KVC_ERR_ARG  # capacity below the list
     assert L.kvc_chunk_plan(None, None, None, 1, 8, 2, 64, 16, N.KVC_I8, 0, None, 0, *map(C.byref, n)) == N.KVC_ERR_ARG
     assert L.kvc_chunk_plan(one.ctypes.data, one.ctypes.data, None, 1, 8, 2, 64, 16, N.KVC_I8, 0, None, 0, None,
-                            C.byref(n[1]), C.byref(n[2])) == N.KVC_ERR_ARG
+                            *map(C.byref, n[1:])) == N.KVC_ERR_ARG
 
 
 @pytest.mark.parametrize("Hq,Hkv,D,block", [(14, 2, 64, 16), (8, 8, 64, 16), (32, 8, 128, 16), (64, 2, 128, 32),
@@ -127,15 +127,15 @@ def test_plan_covers_every_row_and_key_once(Hq, Hkv, D, block, window):
         ql = rng.integers(0 if n > 1 else 1, qmax + 1, n)
         tl = ql + rng.integers(0, tmax, n)
         off = np.concatenate([[0], np.cumsum(-(-tl // block))]) + 5
-        work, nu, nt, nr = ops.chunk_plan(ql, tl, Hq, Hkv, D, block, window=window, tab_off=off)
+        work, nu, nt, (nr, nw) = ops.chunk_plan(ql, tl, Hq, Hkv, D, block, window=window, tab_off=off)
         assert work.shape == (nu, 16) and work[0, 0] == nu and work[0, 1] == nt and work[0, 2] == nr
         start = np.concatenate([[0], np.cumsum(ql)])
         covered = np.zeros((int(ql.sum()), group), np.int64)
         used = np.zeros(nr, bool)
-        spans = {}
+        spans, widened = {}, {}
         tiles = 0
         for e in work[1:]:
-            kind, row, tok, pos, h0, hn, j0, j1, c, nc, rec, tab = e[:12]
+            kind, row, tok, pos, h0, hn, j0, j1, c, nc, rec, tab, wide, wkey, w0, w1 = (int(x) for x in e)
             tiles += kind == 1
             s = int(np.searchsorted(start, row, side="right") - 1)
             assert start[s] <= row and row + tok <= start[s + 1] and pos == tl[s] - ql[s] + row - start[s]
@@ -148,7 +148,16 @@ def test_plan_covers_every_row_and_key_once(Hq, Hkv, D, block, window):
                 r = slice(rec + c * tok * hn, rec + (c + 1) * tok * hn)
                 assert r.stop <= nr and not used[r].any()
                 used[r] = True
-        assert tiles == nt and used.all()
+            if kind == 1:  # its keys lie in the workspace, and it widens its share of them
+                assert wide >= 0 and wkey <= j0 and wide + j1 - wkey <= nw and wkey <= w0 <= w1
+                widened.setdefault((s, wide, wkey), []).append((w0, w1))
+        assert tiles == nt and used.all() and (work[1:nt + 1, 0] == 1).all()
+        rows = np.zeros(nw, np.int64)
+        for (s, wide, wkey), shares in widened.items():
+            for w0, w1 in shares:
+                rows[wide + w0 - wkey:wide + w1 - wkey] += 1
+            assert max(w1 for _, w1 in shares) == tl[s]
+        assert (rows == 1).all()
         for (row, tok, h0, hn), (ranges, first) in spans.items():
             ranges.sort()
             assert ranges[0][0] <= first and all(a[1] == b[0] for a, b in zip(ranges, ranges[1:]))
@@ -159,8 +168,8 @@ def test_plan_covers_every_row_and_key_once(Hq, Hkv, D, block, window):
 
 def test_plan_of_an_empty_batch():
     for q, t in (([], []), ([0, 0], [0, 30])):
-        work, nu, nt, nr = ops.chunk_plan(q, t, 8, 2, 64, 16)
-        assert (nu, nt, nr) == (1, 0, 0) and work[0, 0] == 1
+        work, nu, nt, rows = ops.chunk_plan(q, t, 8, 2, 64, 16)
+        assert (nu, nt, rows) == (1, 0, (0, 0)) and work[0, 0] == 1
 
 
 def test_plain_forms():

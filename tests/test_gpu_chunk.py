@@ -63,7 +63,7 @@ class Batch:
         self.bufs = [dev(self.q), dev(self.pools[0]), dev(self.pools[1]), dev(self.scales), dev(self.table), dev(work)]
         q, k, v, sc, tab, w = self.bufs
         say(f"chunk attention {NAME[self.kv]} N={len(self.ql)} rows={self.rows} Hq={self.Hq} Hkv={self.Hkv} D={D} "
-            f"block={self.block} window={window} cap={cap} units={nu} tiles={nt} records={nr}")
+            f"block={self.block} window={window} cap={cap} units={nu} tiles={nt} workspace rows={nr}")
         ops.paged_chunk_attn(q, out, k, v, None if self.kv == KVC_F16 else sc, tab, len(self.table), w, nu, nt, nr,
                              self.rows, self.Hq, self.Hkv, D, self.block, scale, kv_dtype=self.kv, softcap=cap,
                              window=window, workspace=ws, stream=stream)
@@ -196,7 +196,7 @@ def test_workspaces_streams_and_repeats(kv):
     st = Stream()
     for kw in ({"workspace": None}, {"stream": st.handle}, {"tab_off": False}, {}):
         assert (b.run(**kw) == a).all()
-    assert b.plan[3] > 0
+    assert b.plan[3][0] > 0
 
 
 @pytest.mark.parametrize("kv", ALL, ids=NAME.get)
@@ -228,7 +228,9 @@ def test_captured_launch_replays_other_plans(D, kv):
              Batch([1, 1], [700, 1500], Hq, Hkv, D, block, kv, seed=31, spare=40),
              Batch([60, 1, 1, 1], [1500, 20, 2, 1000], Hq, Hkv, D, block, kv, seed=32, spare=40)]
     want = [b.run() for b in steps]
-    cap = [max(b.plan[i] for b in steps) for i in (1, 2, 3)]
+    tiles = max(b.plan[2] for b in steps)
+    cap = [max(b.plan[1] - b.plan[2] for b in steps) + tiles, tiles,
+           tuple(max(b.plan[3][i] for b in steps) for i in (0, 1))]
     rows = max(b.rows for b in steps)
     size = [max(getattr(b, a).nbytes for b in steps) for a in ("q", "scales", "table")]
     pool = max(b.pools[0].nbytes for b in steps)
