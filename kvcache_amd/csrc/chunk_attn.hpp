@@ -301,12 +301,14 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
     char* vt = kt + Sh::kTile;
     float* s_k = reinterpret_cast<float*>(vt + Sh::kTile);  // factor of a key's score
     float* s_v = s_k + KT;                                   // and of its probability
-    // 16-byte piece of a row in LDS (fp16 V: 32-byte segment)
-    auto piece = [](int r, int c) {
-        if constexpr (Q8) return c ^ (D == 64 ? (r >> 2) & 3 : (r >> 1) & 7);
-        else return c ^ (r & 7);
+    // 16-byte piece of a K row in LDS, and of an 8-bit V row (fp16: 32-byte segment): sixteen rows
+    // of one subtile, and the sixteen (eight) rows that half a wave's transposing read touches, lie
+    // on different banks (64 banks, 256 bytes a cycle)
+    auto piece = [](int r, int c) { return c ^ (ROW == 64 ? (r >> 2) & 3 : ROW == 128 ? (r >> 1) & 7 : r & 15); };
+    auto vseg = [](int r, int seg) {
+        if constexpr (Q8) return seg ^ (D == 64 ? (r >> 2 & 1) | (r >> 3 & 2) : (r >> 1 & 3) | (r >> 2 & 4));
+        else return seg ^ (D == 64 ? (r >> 1) & 3 : r & 7);
     };
-    auto vseg = [](int r, int seg) { return seg ^ (D == 64 ? (r >> 1) & 3 : r & 7); };
 
     Tile T;
     if (kmax > 0) {
@@ -377,7 +379,7 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
                 const int off = i * 1024 + lane * 16;
                 const int r = 16 * h + off / ROW, cb = off % ROW;
                 *reinterpret_cast<u32x4*>(kt + r * ROW + piece(r, cb >> 4) * 16) = T.k[h][i];
-                if constexpr (Q8) *reinterpret_cast<u32x4*>(vt + r * ROW + piece(r, cb >> 4) * 16) = T.v[h][i];
+                if constexpr (Q8) *reinterpret_cast<u32x4*>(vt + r * ROW + vseg(r, cb >> 4) * 16) = T.v[h][i];
                 else *reinterpret_cast<u32x4*>(vt + r * ROW + vseg(r, cb >> 5) * 32 + (cb & 31)) = T.v[h][i];
             }
         __builtin_amdgcn_wave_barrier();
@@ -477,7 +479,7 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
             for (int s = 0; s < SUB / 2; ++s) {
                 if constexpr (Q8) {
                     const int j = n16 >> 1, r = 32 * s + (j < 4 ? 4 * g4 + j : 12 + 4 * g4 + j);
-                    vv[s] = codes_to_f16x8<CT>(ds_read_tr8(vt + r * ROW + piece(r, nt) * 16 + 8 * (n16 & 1)));
+                    vv[s] = codes_to_f16x8<CT>(ds_read_tr8(vt + r * ROW + vseg(r, nt) * 16 + 8 * (n16 & 1)));
                 } else {
                     const int r = 32 * s + 4 * g4 + (n16 >> 2), cb = 8 * (n16 & 3);
                     const s16x4v lo = ds_read_tr16(vt + r * ROW + vseg(r, nt) * 32 + cb);

@@ -25,8 +25,9 @@
 //     keys, and V^T is read back in that order with the transposing LDS read.
 // A wave's scores of the next 32 keys are computed while the exponentials of these are taken.
 //
-// LDS: K rows as 16-byte chunks XOR-permuted by the row, V rows as 32-byte segments permuted by
-// the row, so that neither operand read meets a bank twice.
+// LDS (64 banks, 256 bytes a cycle): K rows as 16-byte chunks permuted so that 16 rows' chunks of one
+// dim range lie on different banks, V rows as 32-byte segments permuted so that the two segments of
+// four rows that half a wave reads do.
 #pragma once
 #include "chunk_attn.hpp"
 
@@ -158,8 +159,8 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
 #pragma unroll
         for (int n = 0; n < VL; ++n) rv[n] = buffer_load16(vr, n * 1024 + lane * 16);
     };
-    auto kchunk = [](int r, int ch) { return ch ^ (r & 7); };
-    auto vseg = [](int r, int seg) { return seg ^ (D == 64 ? (r >> 1) & 3 : r & 7); };
+    auto kchunk = [](int r, int ch) { return ch ^ (D == 64 ? (r >> 1) & 7 : r & 15); };
+    auto vseg = [](int r, int seg) { return seg ^ (D == 64 ? r & 2 : 2 * (r & 3)); };
     bool bad = false;  // this wave cleared elements of V in sets that some row does not see whole
     auto store = [&](int half, bool edge) {
         char* kd = lds.kv[half][0];
@@ -201,9 +202,9 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
 #pragma unroll
         for (int i = 0; i < 16; ++i) O[dt][i] = 0.f;
 
-    int ka[4], va[DT];
+    int ka[KD], va[DT];
 #pragma unroll
-    for (int d = 0; d < 4; ++d) ka[d] = ks * KT * ROW + l32 * ROW + kchunk(l32, 2 * d + h) * 16;
+    for (int d = 0; d < KD; ++d) ka[d] = ks * KT * ROW + l32 * ROW + kchunk(l32, 2 * d + h) * 16;
     const int vr = 4 * h + ((lane & 15) >> 2);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -217,7 +218,7 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
             f32x16 S = C;
 #pragma unroll
             for (int d = 0; d < KD; ++d) {
-                const f16x8v a = *reinterpret_cast<const f16x8v*>(buf + ka[d & 3] + 32 * n * ROW + (d >> 2) * 128);
+                const f16x8v a = *reinterpret_cast<const f16x8v*>(buf + ka[d] + 32 * n * ROW);
                 S = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qb[d], S, 0, 0, 0);
             }
             return S;
