@@ -14,8 +14,7 @@
 // the other half of the LDS buffer; one barrier per set.
 //
 //   S^T[key][row] = K Q^T with v_mfma_f32_32x32x16_f16: a lane holds 16 scores of ONE row
-//     (column l % 32), so a row's maximum needs one exchange with lane l ^ 32.  Widened keys:
-//     the accumulator starts at kBias - reference, so the products' sum is the exponent itself.
+//     (column l % 32), so a row's maximum needs one exchange with lane l ^ 32.
 //   softmax: p = 2^(s - reference + kBias), fp32, then fp16.  The reference lags: it moves to the
 //     row's maximum when a score passes it by more than 2^kLag (and at a row's first key), so p
 //     is at most 2^15, fp16 keeps all its bits down to 2^-21 of the largest, and O is rescaled a
@@ -113,7 +112,6 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     constexpr int DT = D / 32;               // 32-dim output tiles
     constexpr int VL = 16 * ROW / 1024;      // wave loads per 16 rows
     constexpr int kSetBytes = kSetKeys * ROW;
-    constexpr bool direct = WIDE && !CAP;    // the accumulator is the relative score
     static_assert(KS == 1 || KS * QG * 32 * D * 4 <= 2 * 2 * kSetBytes, "partials fit the tile buffers");
     __shared__ float s_ml[KS][QG][32][2];
     __shared__ int s_bad[W];
@@ -189,14 +187,20 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
 #pragma unroll
         for (int d = 0; d < KD; ++d) qb[d] = *reinterpret_cast<const f16x8v*>(q + 16 * d);
     }
+    // paged keys: the score's factor to log2 units, > 0 here (a negative one negates q, exactly; 0: q
+    // becomes 0, so that the -Inf of unseen keys stays one)
+    const float sl2 = WIDE || CAP || p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+    if (!WIDE && !CAP && p.scale_log2 <= 0.f) {
+        const _Float16 f = p.scale_log2 < 0.f ? -1.f : 0.f;
+#pragma unroll
+        for (int d = 0; d < KD; ++d) qb[d] *= f;
+    }
     const int wfirst = u.pos0 + min(32 * qg, u.rows - 1) / u.hn;      // positions of the wave's rows
     const int wlast = u.pos0 + min(32 * qg + 31, u.rows - 1) / u.hn;
 
-    float ref = 0.f, l = 0.f;    // reference of p; sum of the lane's own keys
-    float thr = -FLT_MAX;        // a relative score above it moves the reference (none met yet: any)
-    f32x16 O[DT], C;             // C: what the score accumulator starts from
-#pragma unroll
-    for (int i = 0; i < 16; ++i) C[i] = direct ? kBias : 0.f;
+    float ref = 0.f, l = 0.f;    // p = 2^(score - ref); sum of the lane's own keys
+    float thr = -FLT_MAX;        // a score above it moves the reference (none met yet: any)
+    f32x16 O[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -215,7 +219,9 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
         constexpr bool MASKED = decltype(masked_tag)::value;
         const char* buf = base + half * (2 * kSetBytes);
         auto scores = [&](int n) {
-            f32x16 S = C;
+            f32x16 S;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) S[i] = 0.f;
 #pragma unroll
             for (int d = 0; d < KD; ++d) {
                 const f16x8v a = *reinterpret_cast<const f16x8v*>(buf + ka[d] + 32 * n * ROW);
@@ -226,17 +232,11 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
         // S[i] is key t0 + 32 n + 8 (i / 4) + 4 h + i % 4, seen when low < 32 n + 8 (i / 4) + i % 4 <= lim
         const int lim = min(pos, j1 - 1) - t0 - 4 * h;
         const int low = (p.window > 0 ? pos - p.window : -1) - t0 - 4 * h;
-        // relative scores, those of unseen keys -Inf; the reference moves where one is too far above it
+        // scores in log2 units, those of unseen keys -Inf; the reference moves where one is too far above it
         auto settle = [&](f32x16& S, int n) {
-            if constexpr (!direct) {
-                const float off = kBias - ref;
-                if constexpr (CAP) {
+            if constexpr (CAP) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) S[i] = capped(S[i], WIDE ? 1.f : p.cap_in, p.cap_log2) + off;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) S[i] = __builtin_fmaf(S[i], p.scale_log2, off);
-                }
+                for (int i = 0; i < 16; ++i) S[i] = capped(S[i], WIDE ? 1.f : p.cap_in, p.cap_log2);
             }
             if constexpr (MASKED) {
 #pragma unroll
@@ -248,20 +248,14 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
             float mx = -FLT_MAX;
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[i]);
-            if (__any(mx > thr)) {
-                mx = max_xor32(mx);
+            if (__any(mx * sl2 > thr)) {
+                mx = max_xor32(mx) * sl2;
                 const bool move = mx > thr;
-                const float by = move ? mx - kBias : 0.f;
-                const float corr = move && thr > -FLT_MAX ? fast_exp2(-by) : 1.f;
-                ref += by;
-                thr = move ? kBias + kLag : thr;
+                const float to = move ? mx - kBias : ref;
+                const float corr = thr > -FLT_MAX ? fast_exp2(ref - to) : 1.f;
+                ref = to;
+                thr = move ? mx + kLag : thr;
                 l *= corr;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) S[i] -= by;
-                if constexpr (direct) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) C[i] = kBias - ref;
-                }
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -272,13 +266,13 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
         settle(S, 0);
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-            f32x16 next = C;
+            f32x16 next;
             if (n + 1 < NS) next = scores(n + 1);
             f16x8v pb[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) pb[t][j] = (_Float16)fast_exp2(S[8 * t + j]);
+                for (int j = 0; j < 8; ++j) pb[t][j] = (_Float16)fast_exp2(__builtin_fmaf(S[8 * t + j], sl2, -ref));
                 const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
                 l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 0, 1), one, l, false);
                 l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 2, 3), one, l, false);
