@@ -8,10 +8,12 @@
 // many vector instructions as the softmax has).
 //
 // tile_unit: a workgroup of 8 waves takes 32 QG rows (token, head) of one KV head, QG groups of 32
-// rows times KS = 8 / QG key streams.  Keys come in sets of 128, stream ks of a set taking its 128 /
-// KS keys.  Wave w brings rows 16 w .. + 15 of a set (one block id, whole rows, rows past the end
+// rows times KS = 8 / QG key streams.  Keys come in sets of 64, stream ks of a set taking its 64 /
+// KS keys.  Wave w brings rows 8 w .. + 7 of a set (one block id, whole rows, rows past the end
 // read as zero through the descriptor) into registers while the set before is computed, then into
-// the other half of the LDS buffer; one barrier per set.
+// LDS: two buffers of K, three of V.  The barrier after which a set may be read stands before the
+// last exponentials and P V of the set before it, whose V the next set but one must not overwrite:
+// so a wave always has the scores of the next 32 keys to compute under these exponentials.
 //
 //   S^T[key][row] = K Q^T with v_mfma_f32_32x32x16_f16: a lane holds 16 scores of ONE row
 //     (column l % 32), so a row's maximum needs one exchange with lane l ^ 32.
@@ -22,7 +24,6 @@
 //     probabilities (two a v_dot2), the ones O is made of.
 //   O^T[dim][row] += V^T P^T: the lane's own probabilities are the operand up to the order of
 //     keys, and V^T is read back in that order with the transposing LDS read.
-// A wave's scores of the next 32 keys are computed while the exponentials of these are taken.
 //
 // LDS (64 banks, 256 bytes a cycle): K rows as 16-byte chunks permuted so that 16 rows' chunks of one
 // dim range lie on different banks, V rows as 32-byte segments permuted so that the two segments of
@@ -93,27 +94,28 @@ __global__ __launch_bounds__(256) void widen_kernel(ChunkParams p) {
     }
 }
 
-constexpr int kSetKeys = 128;  // keys of an LDS set: 16 rows for each of 8 waves
+constexpr int kSetKeys = 64;  // keys of an LDS set: 8 rows for each of 8 waves
 
 template <int D>
 struct TileLds {
-    char kv[2][2][kSetKeys * D * 2];  // [half][K / V]
+    char k[2][kSetKeys * D * 2];
+    char v[3][kSetKeys * D * 2];
 };
 
 // WIDE: keys from the workspace (widen_kernel), else from the pages of an fp16 cache.
 template <int D, bool WIDE, int QG, bool CAP>
 __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit& u, TileLds<D>& lds) {
     constexpr int W = 8;
+    constexpr int SR = kSetKeys / W;         // rows of a set that a wave brings
     constexpr int ROW = D * 2;               // bytes of a row
     constexpr int KS = W / QG;               // key streams
     constexpr int KT = kSetKeys / KS;        // keys per stream and set
     constexpr int NS = KT / 32;              // 32-key subtiles
     constexpr int KD = D / 16;               // MFMA k steps over the head dimension
     constexpr int DT = D / 32;               // 32-dim output tiles
-    constexpr int VL = 16 * ROW / 1024;      // wave loads per 16 rows
-    constexpr int kSetBytes = kSetKeys * ROW;
-    static_assert(KS == 1 || KS * QG * 32 * D * 4 <= 2 * 2 * kSetBytes, "partials fit the tile buffers");
-    __shared__ float s_ml[KS][QG][32][2];
+    constexpr int VL = SR * ROW / 1024;      // wave loads per set
+    static_assert(NS >= 1 && KS <= 2, "one or two streams of whole subtiles");
+    __shared__ float s_ml[QG][32][2];
     __shared__ int s_bad[W];
 
     const int lane = threadIdx.x & (kWave - 1);
@@ -134,7 +136,7 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     const int nfull = f1 - f0;
     auto set_at = [&](int i) { return i < nfull ? f0 + i : i - nfull < f0 ? i - nfull : i; };
     // this wave's rows of the i-th set; block ids one set per lane, 64 sets at a time
-    auto first_tok = [&](int i) { return j0 + set_at(i) * kSetKeys + 16 * wave; };
+    auto first_tok = [&](int i) { return j0 + set_at(i) * kSetKeys + SR * wave; };
     int ids = 0;
     auto load_ids = [&](int i) {
         if constexpr (!WIDE) ids = p.table[min(u.tab + (min(first_tok(i + lane), j1 - 1) >> bsh), p.table_len - 1)];
@@ -149,7 +151,7 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
         const int id = WIDE ? 0 : __builtin_amdgcn_readlane(ids, i & (kWave - 1));
         int rows = max(j1 - t, 0);
         asm("" : "+s"(rows));
-        const int bytes = min(rows, 16) * ROW;
+        const int bytes = min(rows, SR) * ROW;
         const size_t off = row_of(rows > 0 ? t : j0, id) * ROW;
         const __amdgpu_buffer_rsrc_t kr = tile_rsrc(kb + off, bytes), vr = tile_rsrc(vb + off, bytes);
 #pragma unroll
@@ -160,9 +162,7 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     auto kchunk = [](int r, int ch) { return ch ^ (D == 64 ? (r >> 1) & 7 : r & 15); };
     auto vseg = [](int r, int seg) { return seg ^ (D == 64 ? r & 2 : 2 * (r & 3)); };
     bool bad = false;  // this wave cleared elements of V in sets that some row does not see whole
-    auto store = [&](int half, bool edge) {
-        char* kd = lds.kv[half][0];
-        char* vd = lds.kv[half][1];
+    auto store = [&](char* kd, char* vd, bool edge) {
         if (edge && any_nonfinite(rv)) {
             clear_nonfinite(rv);
             bad = true;
@@ -170,7 +170,7 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
 #pragma unroll
         for (int n = 0; n < VL; ++n) {
             const int off = n * 1024 + lane * 16;
-            const int r = 16 * wave + off / ROW, cb = off % ROW;
+            const int r = SR * wave + off / ROW, cb = off % ROW;
             *reinterpret_cast<u32x4*>(kd + r * ROW + kchunk(r, cb >> 4) * 16) = rk[n];
             *reinterpret_cast<u32x4*>(vd + r * ROW + vseg(r, cb >> 5) * 32 + (cb & 31)) = rv[n];
         }
@@ -195,8 +195,6 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
 #pragma unroll
         for (int d = 0; d < KD; ++d) qb[d] *= f;
     }
-    const int wfirst = u.pos0 + min(32 * qg, u.rows - 1) / u.hn;      // positions of the wave's rows
-    const int wlast = u.pos0 + min(32 * qg + 31, u.rows - 1) / u.hn;
 
     float ref = 0.f, l = 0.f;    // p = 2^(score - ref); sum of the lane's own keys
     float thr = -FLT_MAX;        // a score above it moves the reference (none met yet: any)
@@ -206,115 +204,120 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
 #pragma unroll
         for (int i = 0; i < 16; ++i) O[dt][i] = 0.f;
 
-    int ka[KD], va[DT];
+    int ka[KD], va[DT];  // operand addresses within a set
 #pragma unroll
-    for (int d = 0; d < KD; ++d) ka[d] = ks * KT * ROW + l32 * ROW + kchunk(l32, 2 * d + h) * 16;
+    for (int d = 0; d < KD; ++d) ka[d] = (ks * KT + l32) * ROW + kchunk(l32, 2 * d + h) * 16;
     const int vr = 4 * h + ((lane & 15) >> 2);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
-        va[dt] = kSetBytes + ks * KT * ROW + vr * ROW + vseg(vr, 2 * dt + ((lane >> 4) & 1)) * 32 + 8 * (lane & 3);
-    const char* base = &lds.kv[0][0][0];
+        va[dt] = (ks * KT + vr) * ROW + vseg(vr, 2 * dt + ((lane >> 4) & 1)) * 32 + 8 * (lane & 3);
 
-    auto compute = [&](int half, int t0, auto masked_tag) {
-        constexpr bool MASKED = decltype(masked_tag)::value;
-        const char* buf = base + half * (2 * kSetBytes);
-        auto scores = [&](int n) {
-            f32x16 S;
+    auto scores = [&](const char* kd, int n) {
+        f32x16 S;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) S[i] = 0.f;
+        for (int i = 0; i < 16; ++i) S[i] = 0.f;
 #pragma unroll
-            for (int d = 0; d < KD; ++d) {
-                const f16x8v a = *reinterpret_cast<const f16x8v*>(buf + ka[d] + 32 * n * ROW);
-                S = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qb[d], S, 0, 0, 0);
-            }
-            return S;
-        };
-        // S[i] is key t0 + 32 n + 8 (i / 4) + 4 h + i % 4, seen when low < 32 n + 8 (i / 4) + i % 4 <= lim
-        const int lim = min(pos, j1 - 1) - t0 - 4 * h;
-        const int low = (p.window > 0 ? pos - p.window : -1) - t0 - 4 * h;
-        // scores in log2 units, those of unseen keys -Inf; the reference moves where one is too far above it
-        auto settle = [&](f32x16& S, int n) {
-            if constexpr (CAP) {
+        for (int d = 0; d < KD; ++d) {
+            const f16x8v a = *reinterpret_cast<const f16x8v*>(kd + ka[d] + 32 * n * ROW);
+            S = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qb[d], S, 0, 0, 0);
+        }
+        return S;
+    };
+    // scores in log2 units, those of unseen keys -Inf; the reference moves where one is too far above
+    // it.  S[i] is key t0 + 8 (i / 4) + 4 h + i % 4.
+    auto settle = [&](f32x16& S, int t0, auto masked_tag) {
+        if constexpr (CAP) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) S[i] = capped(S[i], WIDE ? 1.f : p.cap_in, p.cap_log2);
-            }
-            if constexpr (MASKED) {
+            for (int i = 0; i < 16; ++i) S[i] = capped(S[i], WIDE ? 1.f : p.cap_in, p.cap_log2);
+        }
+        if constexpr (decltype(masked_tag)::value) {
+            // seen when low < 8 (i / 4) + i % 4 <= lim
+            const int lim = min(pos, j1 - 1) - t0 - 4 * h;
+            const int low = (p.window > 0 ? pos - p.window : -1) - t0 - 4 * h;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int c = 32 * n + 8 * (i >> 2) + (i & 3);
-                    S[i] = c <= lim && c > low ? S[i] : -__builtin_inff();
-                }
-            }
-            float mx = -FLT_MAX;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[i]);
-            if (__any(mx * sl2 > thr)) {
-                mx = max_xor32(mx) * sl2;
-                const bool move = mx > thr;
-                const float to = move ? mx - kBias : ref;
-                const float corr = thr > -FLT_MAX ? fast_exp2(ref - to) : 1.f;
-                ref = to;
-                thr = move ? mx + kLag : thr;
-                l *= corr;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) O[dt][i] *= corr;
-            }
-        };
-        f32x16 S = scores(0);
-        settle(S, 0);
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            f32x16 next;
-            if (n + 1 < NS) next = scores(n + 1);
-            f16x8v pb[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) pb[t][j] = (_Float16)fast_exp2(__builtin_fmaf(S[8 * t + j], sl2, -ref));
-                const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
-                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 0, 1), one, l, false);
-                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 2, 3), one, l, false);
-                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 4, 5), one, l, false);
-                l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 6, 7), one, l, false);
-            }
-            // V^T operand: k slots (h, j) are keys 32 n + 16 t + 8 (j / 4) + 4 h + j % 4, of dim 32 dt
-            // + l % 32; two transposing reads of four keys each (16 lanes address four rows of 16
-            // dims: lane i row i / 4, dims 4 (i % 4) .. + 3)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    const char* vt = buf + va[dt] + (32 * n + 16 * t) * ROW;
-                    const s16x4v lo = ds_read_tr16(vt), hi = ds_read_tr16(vt + 8 * ROW);
-                    const f16x8v a = __builtin_bit_cast(f16x8v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                    O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pb[t], O[dt], 0, 0, 0);
-                }
-            if (n + 1 < NS) {
-                settle(next, n + 1);
-                S = next;
+            for (int i = 0; i < 16; ++i) {
+                const int c = 8 * (i >> 2) + (i & 3);
+                S[i] = c <= lim && c > low ? S[i] : -__builtin_inff();
             }
         }
+        float mx = -FLT_MAX;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[i]);
+        if (__any(mx * sl2 > thr)) {
+            mx = max_xor32(mx) * sl2;
+            const bool move = mx > thr;
+            const float to = move ? mx - kBias : ref;
+            const float corr = thr > -FLT_MAX ? fast_exp2(ref - to) : 1.f;
+            ref = to;
+            thr = move ? mx + kLag : thr;
+            l *= corr;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) O[dt][i] *= corr;
+        }
+    };
+    // probabilities and P V of a subtile, the n-th of its set
+    auto weigh = [&](const f32x16& S, const char* vd, int n) {
+        f16x8v pb[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pb[t][j] = (_Float16)fast_exp2(__builtin_fmaf(S[8 * t + j], sl2, -ref));
+            const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
+            l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 0, 1), one, l, false);
+            l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 2, 3), one, l, false);
+            l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 4, 5), one, l, false);
+            l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 6, 7), one, l, false);
+        }
+        // V^T operand: k slots (h, j) are keys 32 n + 16 t + 8 (j / 4) + 4 h + j % 4, of dim 32 dt
+        // + l % 32; two transposing reads of four keys each (16 lanes address four rows of 16
+        // dims: lane i row i / 4, dims 4 (i % 4) .. + 3)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const char* vt = vd + va[dt] + (32 * n + 16 * t) * ROW;
+                const s16x4v lo = ds_read_tr16(vt), hi = ds_read_tr16(vt + 8 * ROW);
+                const f16x8v a = __builtin_bit_cast(f16x8v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pb[t], O[dt], 0, 0, 0);
+            }
     };
 
-    store(0, nfull == 0);
+    store(lds.k[0], lds.v[0], nfull == 0);
     issue(1);
-    // one set: the next one from its registers into the other half of the buffer, the one after
-    // that into flight, then this one's arithmetic
+    __syncthreads();
+    f32x16 S = scores(lds.k[0], 0);
+    settle(S, j0 + set_at(0) * kSetKeys + ks * KT, std::true_type{});
+    // One set, whose first scores are there: the next one from its registers into LDS, the one after
+    // that into flight; then this one's subtiles, each under the scores of the one after it.
+    int v3 = 0;  // the V buffer of the set
     auto set = [&](int i, auto masked_tag) {
-        __syncthreads();
-        store((i + 1) & 1, decltype(masked_tag)::value || i + 1 >= nfull);
+        const char* kd = lds.k[i & 1];
+        char* kn = lds.k[(i + 1) & 1];
+        const char* vd = lds.v[v3];
+        v3 = v3 == 2 ? 0 : v3 + 1;
+        store(kn, lds.v[v3], decltype(masked_tag)::value);
         if (!WIDE && ((i + 2) & (kWave - 1)) == 0) load_ids(i + 2);
         issue(i + 2);  // (sets past the last read nothing: zero-size descriptors)
         const int t0 = j0 + set_at(i) * kSetKeys + ks * KT;
-        if (!decltype(masked_tag)::value ||
-            (32 * qg < u.rows && t0 <= wlast && t0 < j1 && (p.window <= 0 || t0 + KT > wfirst - p.window + 1)))
-            compute(i & 1, t0, masked_tag);
+#pragma unroll
+        for (int n = 0; n + 1 < NS; ++n) {
+            f32x16 next = scores(kd, n + 1);
+            weigh(S, vd, n);
+            settle(next, t0 + 32 * (n + 1), masked_tag);
+            S = next;
+        }
+        __syncthreads();
+        f32x16 next = scores(kn, 0);  // (past the last set: rows that were stored as zero, masked)
+        weigh(S, vd, NS - 1);
+        settle(next, j0 + set_at(i + 1) * kSetKeys + ks * KT, masked_tag);
+        S = next;
     };
-    // (loops of their own: one loop with both forms copied O between them in every set)
+    // sets whose next one is seen whole as well, then the rest (loops of their own: one loop with both
+    // forms copied O between them in every set)
     int i = 0;
-    for (; i < nfull; ++i) set(i, std::false_type{});
+    for (; i < nfull - 1; ++i) set(i, std::false_type{});
     for (; i < nsets; ++i) set(i, std::true_type{});
     l = sum_xor32(l);
     const float m = thr > -FLT_MAX ? ref : -FLT_MAX;
@@ -352,68 +355,49 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     int any_bad = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) any_bad |= s_bad[w];
-    if constexpr (KS == 1) {
-        if (row >= u.rows) return;
+    // two streams: the second one's (m, l, O) go through LDS to the first one's waves
+    static_assert(KS == 1 || QG * 32 * D * 4 <= (int)sizeof(TileLds<D>), "partials fit the buffers");
+    f32x4* part = reinterpret_cast<f32x4*>(&lds) + qg * (DT * 4) * kWave + lane;
+    float M = m, w0 = 1.f, w1 = 0.f;
+    if constexpr (KS == 2) {
+        if (ks == 1) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                f32x4 acc = {O[dt][4 * b], O[dt][4 * b + 1], O[dt][4 * b + 2], O[dt][4 * b + 3]};
-                const int d0 = 32 * dt + 8 * b + 4 * h;
-                if (any_bad) acc = add_bad(acc, d0);
-                write(row, d0, acc, m, l);
+            for (int b = 0; b < DT * 4; ++b)
+                part[b * kWave] = f32x4{O[b >> 2][4 * (b & 3)], O[b >> 2][4 * (b & 3) + 1], O[b >> 2][4 * (b & 3) + 2],
+                                        O[b >> 2][4 * (b & 3) + 3]};
+            if (h == 0) {
+                s_ml[qg][l32][0] = m;
+                s_ml[qg][l32][1] = l;
             }
-    } else {
-        // every stream leaves (m, l, O) in LDS; then wave (qg, ks) combines its share of the
-        // group's dims: slots of four consecutive dims of a column
-        constexpr int SL = DT * 4 / KS;  // slots per wave
-        static_assert(DT * 4 % KS == 0, "slots divide among the streams");
-        f32x4* part = reinterpret_cast<f32x4*>(&lds.kv[0][0][0]);
-        auto slot = [&](int k, int i4) { return part + ((k * QG + qg) * (DT * 4) + i4) * kWave + lane; };
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-                *slot(ks, dt * 4 + b) = f32x4{O[dt][4 * b], O[dt][4 * b + 1], O[dt][4 * b + 2], O[dt][4 * b + 3]};
-        if (h == 0) {
-            s_ml[ks][qg][l32][0] = m;
-            s_ml[ks][qg][l32][1] = l;
         }
         __syncthreads();
-        float M = -FLT_MAX, lt = 0.f;
+        if (ks == 1) return;
+        M = fmaxf(m, s_ml[qg][l32][0]);
+        w0 = fast_exp2(m - M);
+        w1 = fast_exp2(s_ml[qg][l32][0] - M);
+        l = l * w0 + s_ml[qg][l32][1] * w1;
+    }
+    if (row >= u.rows) return;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) M = fmaxf(M, s_ml[k][qg][l32][0]);
-        f32x4 acc[SL];
+    for (int b = 0; b < DT * 4; ++b) {
+        f32x4 acc = {O[b >> 2][4 * (b & 3)], O[b >> 2][4 * (b & 3) + 1], O[b >> 2][4 * (b & 3) + 2], O[b >> 2][4 * (b & 3) + 3]};
+        if constexpr (KS == 2) {
+            const f32x4 x = part[b * kWave];
 #pragma unroll
-        for (int i = 0; i < SL; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            const float wk = fast_exp2(s_ml[k][qg][l32][0] - M);
-            lt = __builtin_fmaf(wk, s_ml[k][qg][l32][1], lt);
-#pragma unroll
-            for (int i = 0; i < SL; ++i) {
-                const f32x4 x = *slot(k, ks * SL + i);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][e] = __builtin_fmaf(wk, x[e], acc[i][e]);
-            }
+            for (int e = 0; e < 4; ++e) acc[e] = acc[e] * w0 + x[e] * w1;
         }
-        if (row >= u.rows) return;
-#pragma unroll
-        for (int i = 0; i < SL; ++i) {
-            const int d0 = 8 * (ks * SL + i) + 4 * h;
-            if (any_bad) acc[i] = add_bad(acc[i], d0);
-            write(row, d0, acc[i], M, lt);
-        }
+        const int d0 = 8 * b + 4 * h;
+        if (any_bad) acc = add_bad(acc, d0);
+        write(row, d0, acc, M, l);
     }
 }
 
 template <int D, bool WIDE, bool CAP>
-__global__ __launch_bounds__(8 * kWave) void chunk_tile_kernel(ChunkParams p) {
+__global__ __launch_bounds__(8 * kWave, D == 64 ? 4 : 2) void chunk_tile_kernel(ChunkParams p) {
     __shared__ __attribute__((aligned(16))) TileLds<D> lds;
     ChunkUnit u;
     if (!chunk_unit(p, u, 0) || u.kind != kKindTile) return;
-    if (u.rows <= 64) tile_unit<D, WIDE, 2, CAP>(p, u, lds);
-    else if (u.rows <= 128) tile_unit<D, WIDE, 4, CAP>(p, u, lds);
+    if (u.rows <= 128) tile_unit<D, WIDE, 4, CAP>(p, u, lds);
     else if (u.rows <= 256) tile_unit<D, WIDE, 8, CAP>(p, u, lds);
 }
 
