@@ -42,41 +42,125 @@ struct PlanUnit {
     long long cost;
 };
 
-// The batch as units.  A sequence whose new tokens make more than kStreamRows rows of a KV head
-// is cut into tiles of many rows, others into units of 16.
-constexpr int kStreamRows = 32;
-constexpr int kChunkKeys = 1024;
+// Keys per chunk of the units of 16 rows, `keys` of them over all units and KV heads.  Two
+// workgroups fit a CU (512), and chunks of 512 keys keep them in flight; below that a batch is
+// still cut for one workgroup a CU down to 256 keys (one round of four waves).  int8, 32q/8kv, D
+// 128: one sequence of 4000 38.4 us whole, 15.2 in chunks of 1024, 9.1 in 256; 64 of 32..4096 43.4
+// whole, 34.6 for 256 workgroups, 30.8 for 512; 16 of 4000 (8q/8kv, D 64) 33 whole, 24.1 and 22.9.
+// At most 32 chunks of a sequence, whose merge grows with them (one of 20000, 8q/8kv: 14.1 us in 40
+// chunks, 13.4 in 32, 17.5 in 63).
+long long stream_chunk(long long keys, int longest) {
+    const long long one = (keys + 255) / 256, two = (keys + 511) / 512;
+    const long long c = std::max(256LL, std::min(one, std::max(two, 512LL)));
+    return (std::max<long long>(c, (longest + 31) / 32) + 63) / 64 * 64;
+}
+
+// Chunks of `len` keys at a target of c (up to 1.5 c stay whole).
+int chunks_of(long long len, long long c) { return len > c * 3 / 2 ? (int)((len + c - 1) / c) : 1; }
+
+// Keys per chunk of the tiles (INT_MAX: whole): the shortest estimate among whole tiles and chunks
+// for one, two or three rounds of the card's workgroups.  A set of 64 keys takes a tile of 256 rows
+// 2.1 us at head_dim 128 (one workgroup a CU), 1.8 at 64 (two a CU), a unit another 4; the partials
+// are written and read at about 4 TB/s and merged by a launch of 4 us.  2000 tokens of 32 heads
+// behind 4000, D 128 (256 workgroups whole): 103 us whole, 125 in 320 workgroups.
+long long tile_chunk(const std::vector<Tile>& tiles, int Hkv, int D) {
+    long long keys = 0, longest = 0, rows_keys = 0, n = 0;
+    for (const Tile& t : tiles) {
+        if (t.kind != kKindTile) continue;
+        const long long len = t.j1 - t.j0;
+        keys += len;
+        longest = std::max(longest, len);
+        rows_keys += t.ntok * t.hn;
+        ++n;
+    }
+    if (n == 0) return INT_MAX;
+    const double per_key = (D == 128 ? 2.1 : 1.8) / 64, unit = 4.0;
+    const long long slots = D == 128 ? 256 : 512;
+    auto units = [&](long long c) {
+        long long u = 0;
+        for (const Tile& t : tiles)
+            if (t.kind == kKindTile) u += chunks_of(t.j1 - t.j0, c);
+        return u * Hkv;
+    };
+    auto estimate = [&](long long c) {
+        const long long u = units(c);
+        const double mean = (double)keys * Hkv / u, top = (double)std::min(longest, c * 3 / 2);
+        const double rounds = (double)((u + slots - 1) / slots);
+        double t = u <= slots ? unit + per_key * top
+                              : std::min(rounds * (unit + per_key * top),
+                                         std::max(rounds * (unit + per_key * mean), (u * unit + per_key * keys * Hkv) / slots +
+                                                                                        0.4 * (unit + per_key * top)));
+        if (u > n * Hkv) t += 4.0 + 8.0 * rows_keys * Hkv * D * ((double)u / (n * Hkv)) / 4e6;
+        return t;
+    };
+    long long best = INT_MAX;
+    double least = estimate(INT_MAX / 2);
+    for (int k = 1; k <= 3; ++k) {
+        long long c = std::max(512LL, (keys * Hkv + k * slots - 1) / (k * slots));
+        for (int i = 0; i < 40 && c < longest && units(c) > k * slots; ++i) c += c / 16 + 1;
+        c = (c + 63) / 64 * 64;
+        if (c >= longest) continue;
+        const double t = estimate(c);
+        if (t < 0.97 * least) least = t, best = c;
+    }
+    return best;
+}
+
+// The batch as units.  Where the sequences of more than kTileRows rows (token, head) of a KV head
+// make enough work, they are cut into tiles of up to 256 rows; all else into units of 16.
+constexpr int kTileRows = 64;
 void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N, int Hq, int Hkv, int D, int BLOCK,
                 int kv_dtype, int window, std::vector<PlanUnit>& units, long long& records, long long& wide) {
     const int group = Hq / Hkv;
-    const bool matrix = matrix_path(D, BLOCK);
+    auto first_key = [&](int pos) { return window > 0 ? std::max(0, pos - window + 1) / 64 * 64 : 0; };
+    // Tiles reach about three times the rate of units of 16 rows, but take a launch more, 8-bit caches
+    // two (widening).  One sequence, int8 (fp16), units of 16 and tiles: 14q/2kv, D 64, 400 tokens
+    // behind 1000 (1.7 GFLOP) 17 and 19 us (15 and 16), 1000 behind 1000 (5.4) 30 and 30 (26 and 25),
+    // 400 behind 4000 (6.0) 36 and 31 (32 and 25); 32q/8kv, D 128, 64 behind 4000 (4.2) 24 and 27 (23
+    // and 19), 400 behind 1000 (7.9) 38 and 35 (37 and 30), 150 behind 4000 (10) 50 and 39 (48 and 31).
+    bool tiled = false;
+    if (matrix_path(D, BLOCK)) {
+        double flops = 0;
+        for (int s = 0; s < N; ++s)
+            if ((long long)q_lens[s] * group > kTileRows) {
+                const double n = q_lens[s], seen = kv_lens[s] - n + 0.5 * (n + 1);
+                flops += 4.0 * D * Hq * n * (window > 0 ? std::min<double>(seen, window) : seen);
+            }
+        tiled = flops >= (D == 64 ? 5e9 : 7e9) * (kv_dtype == KVC_F16 ? 0.6 : 1.0);
+    }
     std::vector<Tile> tiles;
-    long long row = 0, tab = 0;
+    long long row = 0, tab = 0, stream_keys = 0;
+    int stream_longest = 0;
     wide = 0;
     for (int s = 0; s < N; ++s) {
         const int nq = q_lens[s], nk = kv_lens[s];
         if (tab_off) tab = tab_off[s];
-        // the first key that any of the new tokens sees
-        const int key0 = window > 0 ? std::max(0, nk - nq - window + 1) / 64 * 64 : 0;
-        const bool many = matrix && (long long)nq * group > kStreamRows;
-        const int cap = !many ? 16 : (long long)nq * group <= 64 ? 64 : (long long)nq * group <= 1024 ? 128 : 256;
+        const long long rows = (long long)nq * group;
+        const bool tile = tiled && rows > kTileRows;
+        const int cap = !tile ? 16 : rows <= 128 ? 128 : 256;
         const int hstep = std::min(group, cap), tstep = std::max(1, cap / group);
+        const int key0 = first_key(nk - nq);  // the first key that any of the new tokens sees
         for (int i = 0; i < nq; i += tstep)
             for (int h = 0; h < group; h += hstep) {
-                Tile t{many ? kKindTile : kKindRows, (int)row + i, std::min(tstep, nq - i), nk - nq + i, h,
+                Tile t{tile ? kKindTile : kKindRows, (int)row + i, std::min(tstep, nq - i), nk - nq + i, h,
                        std::min(hstep, group - h), 0, 0, (int)tab, (int)std::min<long long>(wide, INT_MAX), key0};
                 t.j1 = t.pos0 + t.ntok;
-                t.j0 = window > 0 ? std::max(0, t.pos0 - window + 1) / 64 * 64 : 0;
+                t.j0 = first_key(t.pos0);
+                if (!tile) {
+                    stream_keys += t.j1 - t.j0;
+                    stream_longest = std::max(stream_longest, t.j1 - t.j0);
+                }
                 tiles.push_back(t);
             }
-        if (many && kv_dtype != KVC_F16) wide += nk - key0;
+        if (tile && kv_dtype != KVC_F16) wide += nk - key0;
         row += nq;
         if (!tab_off) tab += ((long long)nk + BLOCK - 1) / BLOCK;
     }
     records = 0;
+    const long long chunk[2] = {stream_chunk(stream_keys * Hkv, stream_longest), tile_chunk(tiles, Hkv, D)};
     for (const Tile& t : tiles) {
         const int len = t.j1 - t.j0;
-        int nc = t.kind == kKindTile ? 1 : std::max(1, (len + kChunkKeys - 1) / kChunkKeys);
+        int nc = chunks_of(len, chunk[t.kind == kKindTile]);
         const int step = ((len + nc - 1) / nc + 63) / 64 * 64;
         nc = (len + step - 1) / step;
         const int rows = t.ntok * t.hn;
@@ -145,20 +229,22 @@ int launch_chunks_d(const ChunkParams& p, int n_tiles, hipStream_t st) {
                 const int rc = hip_check(hipGetLastError(), "chunk attention widening launch");
                 if (rc) return rc;
             }
-            const dim3 grid(tiles * Hkv), block(8 * kWave);
+            const dim3 grid(tiles * Hkv), block(kTileWaves * kWave);
             if (p.cap_log2 > 0.f) hipLaunchKernelGGL((chunk_tile_kernel<D, kWide, true>), grid, block, 0, st, p);
             else hipLaunchKernelGGL((chunk_tile_kernel<D, kWide, false>), grid, block, 0, st, p);
             const int rc = hip_check(hipGetLastError(), "chunk attention tile launch");
             if (rc) return rc;
         }
         if (matrix && units > tiles)
-            hipLaunchKernelGGL((chunk_stream_kernel<D, CT>), dim3((units - tiles) * Hkv),
-                               dim3(StreamShape<D, CT>::W * kWave), 0, st, p);
+            hipLaunchKernelGGL((chunk_stream_kernel<D, CT>), dim3((units - tiles) * Hkv), dim3(kStreamWaves * kWave), 0, st, p);
     }
     if (!matrix) hipLaunchKernelGGL((chunk_rows_kernel<D, CT>), dim3(units * Hkv), dim3(256), 0, st, p);
     int rc = hip_check(hipGetLastError(), "chunk attention launch");
     if (rc || p.n_records == 0) return rc;
-    hipLaunchKernelGGL((merge_chunks_kernel<D>), dim3(units * Hkv), dim3(256), 0, st, p);
+    // a workgroup's share of the rows in about one pass
+    const long long passes = ((long long)p.n_records * (D / 4) + 256LL * units - 1) / (256LL * units);
+    hipLaunchKernelGGL((merge_chunks_kernel<D>), dim3(units * Hkv, (unsigned)std::min(8LL, std::max(1LL, passes))), dim3(256),
+                       0, st, p);
     return hip_check(hipGetLastError(), "chunk attention merge launch");
 }
 

@@ -206,6 +206,8 @@ __global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkParams p) {
 // touches at the same piece lie on different banks.
 constexpr int kProbBits = 15;  // probabilities (times V scales) go up to 2^15
 
+constexpr int kStreamWaves = 4;  // waves of a workgroup
+
 template <int D, int CT>
 struct StreamShape {
     static constexpr int CB = kCodeBytes<CT>;
@@ -216,7 +218,7 @@ struct StreamShape {
     static constexpr int KD = D / 32;               // k steps over the head dimension
     static constexpr int NT = D / 16;               // 16-dim output tiles
     static constexpr int kTile = KT * ROW;          // bytes of a K (or V) tile
-    static constexpr int W = D == 64 ? 8 : 4;       // waves of a workgroup
+    static constexpr int W = kStreamWaves;
     // per wave: the K and V tiles, and the keys' factors
     static constexpr int kWaveBytes = 2 * kTile + 2 * KT * 4;
     static constexpr int kBytes = W * kWaveBytes;
@@ -577,7 +579,7 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
 }
 
 template <int D, int CT>
-__global__ __launch_bounds__((StreamShape<D, CT>::W * kWave), (D == 64 ? 4 : 2)) void chunk_stream_kernel(ChunkParams p) {
+__global__ __launch_bounds__(kStreamWaves * kWave, D == 64 ? 4 : 2) void chunk_stream_kernel(ChunkParams p) {
     __shared__ __attribute__((aligned(16))) char lds[StreamShape<D, CT>::kBytes];
     ChunkUnit u;
     if (!chunk_unit(p, u, max(p.work[kHdrTiles], 0)) || u.kind != kKindRows) return;
@@ -585,66 +587,50 @@ __global__ __launch_bounds__((StreamShape<D, CT>::W * kWave), (D == 64 ? 4 : 2))
 }
 
 // Partial rows of the units with nc > 1 as output rows: out = sum_c 2^(m_c - M) acc_c / sum_c
-// 2^(m_c - M) l_c.  A tile's nc units take its rows in turn, one at a time: 256 / (D / 4) chunks
-// side by side (a thread four dims of one), each thread over its chunks, then across them in LDS.
+// 2^(m_c - M) l_c.  A thread takes four dims of a row over all its chunks, eight of them in flight;
+// the workgroups of a tile's nc units (times gridDim.y) share its rows.
 template <int D>
 __global__ __launch_bounds__(256) void merge_chunks_kernel(ChunkParams p) {
-    constexpr int TD = D / 4, SLOTS = 256 / TD;
-    __shared__ f32x4 s_acc[SLOTS][TD];
-    __shared__ float s_ml[SLOTS][2];
+    constexpr int TD = D / 4, E = 8;
     ChunkUnit u;
     if (!chunk_unit(p, u, 0) || u.nc == 1) return;
-    const int slot = threadIdx.x / TD, d = threadIdx.x % TD * 4;
-    const int n = min(SLOTS, u.nc);
-    for (int r = u.c; r < u.rows; r += u.nc) {
-        const size_t rec0 = (size_t)u.hk * p.n_records + u.rec0 + r;
+    const size_t head = (size_t)u.hk * p.n_records + u.rec0;
+    for (int i = (blockIdx.y * u.nc + u.c) * 256 + threadIdx.x; i < u.rows * TD; i += gridDim.y * u.nc * 256) {
+        const int r = i / TD, d = i % TD * 4;
         float M = -FLT_MAX, l = 0.f;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        // four chunks in flight (past the count the last one's again, with weight 0)
-        for (int c = slot; c < u.nc; c += 4 * SLOTS) {
-            float m[4], lc[4];
-            f32x4 a[4];
+        for (int c0 = 0; c0 < u.nc; c0 += E) {
+            // (past the count the last chunk's again, with weight 0)
+            f32x2 ml[E];
+            f32x4 a[E];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const size_t rec = rec0 + (size_t)min(c + i * SLOTS, u.nc - 1) * u.rows;
-                m[i] = p.part_ml[rec * 2];
-                lc[i] = p.part_ml[rec * 2 + 1];
-                a[i] = *reinterpret_cast<const f32x4*>(p.part_acc + rec * D + d);
+            for (int e = 0; e < E; ++e) {
+                const size_t rec = head + (size_t)min(c0 + e, u.nc - 1) * u.rows + r;
+                ml[e] = *reinterpret_cast<const f32x2*>(p.part_ml + rec * 2);
+                a[e] = *reinterpret_cast<const f32x4*>(p.part_acc + rec * D + d);
             }
+            float top = M;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (c + i * SLOTS >= u.nc) continue;
-                const float mn = fmaxf(M, m[i]), w0 = fast_exp2(M - mn), w1 = fast_exp2(m[i] - mn);
-                M = mn;
-                l = l * w0 + lc[i] * w1;
+            for (int e = 0; e < E; ++e) top = fmaxf(top, ml[e][0]);
+            const float w0 = fast_exp2(M - top);
+            M = top;
+            l *= w0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[e] = acc[e] * w0 + a[i][e] * w1;
+            for (int k = 0; k < 4; ++k) acc[k] *= w0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (c0 + e >= u.nc) continue;
+                const float w = fast_exp2(ml[e][0] - M);
+                l = __builtin_fmaf(w, ml[e][1], l);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] = __builtin_fmaf(w, a[e][k], acc[k]);
             }
         }
-        s_acc[slot][threadIdx.x % TD] = acc;
-        if (d == 0) {
-            s_ml[slot][0] = M;
-            s_ml[slot][1] = l;
-        }
-        __syncthreads();
-        if (threadIdx.x < TD) {
-            float Mt = -FLT_MAX, lt = 0.f;
-            f32x4 at = {0.f, 0.f, 0.f, 0.f};
-            for (int i = 0; i < n; ++i) Mt = fmaxf(Mt, s_ml[i][0]);
-            for (int i = 0; i < n; ++i) {
-                const float w = fast_exp2(s_ml[i][0] - Mt);
-                lt = __builtin_fmaf(w, s_ml[i][1], lt);
-                const f32x4 x = s_acc[i][threadIdx.x];
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        f16x4 o;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) at[e] = __builtin_fmaf(w, x[e], at[e]);
-            }
-            const float inv = lt == 0.f ? 0.f : 1.0f / lt;
-            f16x4 o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = (_Float16)(at[e] * inv);
-            *reinterpret_cast<f16x4*>(p.out + chunk_row(p, u, r, D) + d) = o;
-        }
-        __syncthreads();
+        for (int k = 0; k < 4; ++k) o[k] = (_Float16)(acc[k] * inv);
+        *reinterpret_cast<f16x4*>(p.out + chunk_row(p, u, r, D) + d) = o;
     }
 }
 
