@@ -86,7 +86,9 @@ int         kvc_device_count(int* count);
  * "self_prefetch_xcd" (1: each KV head's slice is read ahead on the XCD whose
  * units read it), "self_lead_tokens" (self-planned launches on the VALU kernel: a
  * sequence of at most this many tokens is attended whole while the kernel plans the
- * others, default 320, 0 = none; at most the largest chunk).
+ * others, default 320, 0 = none; at most the largest chunk), "chunk_tiles"
+ * (kvc_chunk_plan: sequences with more than 64 rows per KV head as tiles of many
+ * rows, -1 where the batch's work carries their launches, 0 never, 1 always).
  * The matrix-core path takes fp16 K/V, head_dim 64 or 128, 3..16 query heads per
  * KV head and, paged, a power-of-two BLOCK >= 16; other shapes use the VALU
  * kernels. */
@@ -414,7 +416,7 @@ int kvc_read_kv(void* k, void* v, const void* k_pool, const void* v_pool, const 
  *   over an 8-bit cache hold as fp16 in the workspace.  host_tab_off (N + 1, NULL: tables packed
  *   in sequence order) locates each sequence's table in table_all.  The caller copies the list
  *   to the device.
- * kvc_paged_chunk_attn: runs it (same shape, kv_dtype and window; tuning knobs play no part).
+ * kvc_paged_chunk_attn: runs it (same shape, kv_dtype and window; tuning knobs play no part here).
  *   Every table read is bounded by table_len, every row by rows.  n_tiles, n_units - n_tiles,
  *   n_records and n_wide may exceed the list's own counts: a captured graph replays any list
  *   within them that is copied to the same address.  workspace: kvc_chunk_workspace_size bytes

@@ -1515,6 +1515,7 @@ int kvc_set_tuning(const char* key, int value) {
     else if (k == "self_prefetch_xcd" && (value == 0 || value == 1)) tuning().self_prefetch_xcd = value;
     else if (k == "self_lead_tokens" && value >= 0) tuning().self_lead_tokens = value;
     else if (k == "chain_spin" && value >= 0) tuning().chain_spin = value;
+    else if (k == "chunk_tiles" && value >= -1 && value <= 1) tuning().chunk_tiles = value;
     else return set_error(KVC_ERR_ARG, "unknown tuning key or bad value: " + k);
     return KVC_OK;
 }
@@ -1539,6 +1540,7 @@ int kvc_get_tuning(const char* key, int* value) {
     else if (k == "self_prefetch_xcd") *value = tuning().self_prefetch_xcd;
     else if (k == "self_lead_tokens") *value = tuning().self_lead_tokens;
     else if (k == "chain_spin") *value = tuning().chain_spin;
+    else if (k == "chunk_tiles") *value = tuning().chunk_tiles;
     else return set_error(KVC_ERR_ARG, "unknown tuning key: " + k);
     return KVC_OK;
 }

@@ -15,6 +15,7 @@ size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 size_t acc_bytes(int Hkv, int D, int n_records) { return up((size_t)Hkv * n_records * D * sizeof(float), kPartAlign); }
 size_t wide_bytes(int Hkv, int D, int n_wide) { return up((size_t)Hkv * n_wide * D * 2, kPartAlign); }
 size_t ml_bytes(int Hkv, int n_records) { return up((size_t)Hkv * n_records * 2 * sizeof(float), kPartAlign); }
+size_t factor_bytes(int Hkv, int n_wide) { return up((size_t)Hkv * n_wide * sizeof(float), kPartAlign); }
 
 int check_shape(int Hq, int Hkv, int D, int BLOCK, int kv_dtype, int window) {
     if (kv_dtype == KVC_F32) return set_error(KVC_ERR_UNSUPPORTED, "the cache must be KVC_F16, KVC_I8 or KVC_E4M3");
@@ -126,7 +127,8 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
                 const double n = q_lens[s], seen = kv_lens[s] - n + 0.5 * (n + 1);
                 flops += 4.0 * D * Hq * n * (window > 0 ? std::min<double>(seen, window) : seen);
             }
-        tiled = flops >= (D == 64 ? 5e9 : 7e9) * (kv_dtype == KVC_F16 ? 0.6 : 1.0);
+        const int knob = tuning().chunk_tiles;
+        tiled = knob >= 0 ? knob == 1 : flops >= (D == 64 ? 5e9 : 7e9) * (kv_dtype == KVC_F16 ? 0.6 : 1.0);
     }
     std::vector<Tile> tiles;
     long long row = 0, tab = 0, stream_keys = 0;
@@ -304,7 +306,7 @@ size_t kvc_chunk_workspace_size(int Hq, int Hkv, int D, int n_records, int n_wid
     if (Hq <= 0 || Hkv <= 0 || D <= 0) return 0;
     n_records = std::max(n_records, 0);
     n_wide = std::max(n_wide, 0);
-    return acc_bytes(Hkv, D, n_records) + ml_bytes(Hkv, n_records) + 2 * wide_bytes(Hkv, D, n_wide);
+    return acc_bytes(Hkv, D, n_records) + ml_bytes(Hkv, n_records) + 2 * wide_bytes(Hkv, D, n_wide) + factor_bytes(Hkv, n_wide);
 }
 
 int kvc_paged_chunk_attn(const void* q, void* out, const void* k_pool, const void* v_pool, const float* kv_scales,
@@ -357,7 +359,9 @@ int kvc_paged_chunk_attn(const void* q, void* out, const void* k_pool, const voi
             p.part_ml = reinterpret_cast<float*>(ws);
             ws += ml_bytes(Hkv, n_records);
             p.wide_k = reinterpret_cast<_Float16*>(ws);
-            p.wide_v = reinterpret_cast<_Float16*>(ws + wide_bytes(Hkv, D, n_wide));
+            ws += wide_bytes(Hkv, D, n_wide);
+            p.wide_v = reinterpret_cast<_Float16*>(ws);
+            p.wide_f = reinterpret_cast<float*>(ws + wide_bytes(Hkv, D, n_wide));
         }
         const hipStream_t st = (hipStream_t)stream;
         switch (D) {

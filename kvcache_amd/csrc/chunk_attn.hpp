@@ -39,6 +39,7 @@ struct ChunkParams {
     float* part_ml;         // [Hkv][n_records][2]
     _Float16* wide_k;       // [Hkv][n_wide][D]
     _Float16* wide_v;
+    float* wide_f;          // [Hkv][n_wide]: the score's factor
 };
 
 namespace {
@@ -451,7 +452,8 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
             for (int i = 0; i < 4 * SUB; ++i) mx = seen(i) ? fmaxf(mx, S[a][i >> 2][i & 3]) : mx;
             mx = max_xor32(max_xor16(mx));
             const float mn = fmaxf(m[a], mx), corr = fast_exp2(m[a] - mn);
-            const float ref = Q8 ? mn : mn - (float)kProbBits;
+            // (a little further for scores whose last bit is more than 1: p has to stay below 2^16)
+            const float ref = Q8 ? mn : mn - (float)kProbBits + fabsf(mn) * 0x1p-23f;
             float ps = 0.f;
             fence();
 #pragma unroll

@@ -1,11 +1,15 @@
 // chunk_tile.hpp -- chunk attention of many rows on the matrix cores (head_dim 64 / 128).
 //
-// 8-bit caches: widen_kernel first turns the keys that tiles see into fp16 rows in the workspace,
-// K times its scale and the factor to log2 units, V times its scale, each product rounded once
-// (what an fp16 cache would hold; values beyond fp16's range, 65504, become Inf).  Every tile of a
-// sequence reads all of its keys, so widening them in the tiles costs the more the more tiles
-// there are: 2000 tokens of 32 heads behind 6000, D 128, were 316 us with it in the tiles (about as
-// many vector instructions as the softmax has).
+// 8-bit caches: widen_kernel first turns the keys that tiles see into fp16 rows in the workspace.  Every
+// tile of a sequence reads all of its keys, so widening them in the tiles costs the more the more
+// tiles there are: 2000 tokens of 32 heads behind 6000, D 128, were 316 us with it in the tiles (about
+// as many vector instructions as the softmax has).  An error of a score grows with the score, so K is
+// exact: the rows hold the code times the leading bits of its scale, as many as fp16 has room for
+// behind the code's (4 for int8, 7 for e4m3); the rest of the scale goes in fp32 to the score.  V is
+// its code times its scale, rounded once (what an fp16 cache would hold; values beyond fp16's range,
+// 65504, become Inf).  Error against 64 bits there 3.0e-4, the output's own rounding 2.1e-4; K rounded
+// like V gave 5.0e-4 in 252 instead of 272 us, V exact as well 2.9e-4 in 280 (two multiplications per
+// score instead of one).
 //
 // tile_unit: a workgroup of 8 waves takes 32 QG rows (token, head) of one KV head, QG groups of 32
 // rows times KS = 8 / QG key streams.  Keys come in sets of 64, stream ks of a set taking its 64 /
@@ -37,8 +41,8 @@ namespace {
 constexpr float kBias = 7.f, kLag = 8.f;
 
 // Sixteen codes times s as fp16, each rounded once.  int8: the fp16 1024 + (c + 128) comes from a
-// byte permutation, and one fma takes 1152 s off again; s has 20 bits (row_factor), so that 1152 s
-// is exact.
+// byte permutation, and one fma takes 1152 s off again; s has 20 bits at most (leading), so that
+// 1152 s is exact.
 template <int CT>
 __device__ __forceinline__ void scaled_f16(u32x4 c, float s, u32x4 (&out)[2]) {
     const float off = CT == kCacheI8 ? -1152.f * s : 0.f;
@@ -63,7 +67,8 @@ __device__ __forceinline__ void scaled_f16(u32x4 c, float s, u32x4 (&out)[2]) {
     }
 }
 
-__device__ __forceinline__ float row_factor(float s) { return __uint_as_float(__float_as_uint(s) & 0xFFFFFFF0u); }
+// s without all but its leading `bits` bits
+__device__ __forceinline__ float leading(float s, int bits) { return __uint_as_float(__float_as_uint(s) & (~0u << (24 - bits))); }
 
 // A tile's share of its sequence's keys, as fp16 rows of the workspace.
 constexpr int kWidenBlocks = 16;  // workgroups per tile and KV head
@@ -80,17 +85,32 @@ __global__ __launch_bounds__(256) void widen_kernel(ChunkParams p) {
         const int b = k / p.block;
         const int id = p.table[min(u.tab + b, p.table_len - 1)];
         const size_t row = ((size_t)(unsigned)(id * p.Hkv + u.hk)) * p.block + (k - b * p.block);
-        const size_t to = ((size_t)u.hk * p.n_wide + u.wide + (k - u.wkey)) * D + 16 * l;
+        const size_t to = (size_t)u.hk * p.n_wide + u.wide + (k - u.wkey);
         const f32x2 s = *reinterpret_cast<const f32x2*>(p.scales + row * 2);
         const u32x4 ck = *reinterpret_cast<const u32x4*>(static_cast<const char*>(p.k) + row * D + 16 * l);
         const u32x4 cv = *reinterpret_cast<const u32x4*>(static_cast<const char*>(p.v) + row * D + 16 * l);
+        u32x4* ko = reinterpret_cast<u32x4*>(p.wide_k + to * D + 16 * l);
+        u32x4* vo = reinterpret_cast<u32x4*>(p.wide_v + to * D + 16 * l);
+        const float lead = leading(s[0], CT == kCacheI8 ? 4 : 7);
         u32x4 x[2];
-        scaled_f16<CT>(ck, row_factor(s[0] * kf), x);
-        reinterpret_cast<u32x4*>(p.wide_k + to)[0] = x[0];
-        reinterpret_cast<u32x4*>(p.wide_k + to)[1] = x[1];
-        scaled_f16<CT>(cv, row_factor(s[1]), x);
-        reinterpret_cast<u32x4*>(p.wide_v + to)[0] = x[0];
-        reinterpret_cast<u32x4*>(p.wide_v + to)[1] = x[1];
+        scaled_f16<CT>(ck, lead, x);
+        ko[0] = x[0];
+        ko[1] = x[1];
+        scaled_f16<CT>(cv, leading(s[1], 20), x);
+        vo[0] = x[0];
+        vo[1] = x[1];
+        // (0, subnormal and non-finite scales: all of it is in K)
+        if (l == 0) p.wide_f[to] = fabsf(lead) >= FLT_MIN && fabsf(lead) <= FLT_MAX ? s[0] / lead * kf : kf;
+    }
+}
+
+// S[i] times the f of lane i of the 16 around a lane (one instruction each: a row broadcast is an
+// operand's modifier).
+template <int I = 0>
+__device__ __forceinline__ void scale_scores(f32x16& S, float f) {
+    if constexpr (I < 16) {
+        S[I] *= __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, f), 0x150 + I, 0xf, 0xf, true));
+        scale_scores<I + 1>(S, f);
     }
 }
 
@@ -101,6 +121,7 @@ template <int D>
 struct TileLds {
     char k[2][kSetKeys * D * 2];
     char v[3][kSetKeys * D * 2];
+    float kf[3][kSetKeys];  // widened keys: the score's factor
 };
 
 // WIDE: keys from the workspace (widen_kernel), else from the pages of an fp16 cache.
@@ -147,6 +168,7 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
         else return (((size_t)(unsigned)(id * p.Hkv + u.hk)) << bsh) + (t & bmask);
     };
     u32x4 rk[VL], rv[VL];
+    float rf = 0.f;  // (of row 8 w + lane, lanes 0 .. 7)
     auto issue = [&](int i) {
         const int t = first_tok(i);
         const int id = WIDE ? 0 : __builtin_amdgcn_readlane(ids, i & (kWave - 1));
@@ -159,11 +181,18 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
         for (int n = 0; n < VL; ++n) rk[n] = buffer_load16(kr, n * 1024 + lane * 16);
 #pragma unroll
         for (int n = 0; n < VL; ++n) rv[n] = buffer_load16(vr, n * 1024 + lane * 16);
+        if constexpr (WIDE) {
+            const __amdgpu_buffer_rsrc_t fr = tile_rsrc(p.wide_f + off / ROW, min(rows, SR) * 4);
+            rf = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(fr, lane * 4, 0, 0));
+        }
     };
     auto kchunk = [](int r, int ch) { return ch ^ (D == 64 ? (r >> 1) & 7 : r & 15); };
     auto vseg = [](int r, int seg) { return seg ^ (D == 64 ? r & 2 : 2 * (r & 3)); };
     bool bad = false;  // this wave cleared elements of V in sets that some row does not see whole
-    auto store = [&](char* kd, char* vd, bool edge) {
+    auto store = [&](int kb2, int vb3, bool edge) {
+        char* kd = lds.k[kb2];
+        char* vd = lds.v[vb3];
+        if (WIDE && lane < SR) lds.kf[vb3][SR * wave + lane] = rf;
         if (edge && any_nonfinite(rv)) {
             clear_nonfinite(rv);
             bad = true;
@@ -224,9 +253,11 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
         }
         return S;
     };
+    const int fl = 8 * ((lane & 15) >> 2) + 4 * h + (lane & 3);  // the key whose factor a lane fetches
     // scores in log2 units, those of unseen keys -Inf; the reference moves where one is too far above
-    // it.  S[i] is key t0 + 8 (i / 4) + 4 h + i % 4.
-    auto settle = [&](f32x16& S, int t0, auto masked_tag) {
+    // it.  S[i] is key t0 + 8 (i / 4) + 4 h + i % 4; the subtile's factors begin at kf.
+    auto settle = [&](f32x16& S, const float* kf, int t0, auto masked_tag) {
+        if constexpr (WIDE) scale_scores(S, kf[fl]);
         if constexpr (CAP) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) S[i] = capped(S[i], WIDE ? 1.f : p.cap_in, p.cap_log2);
@@ -248,7 +279,8 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
         if (__builtin_expect(__any(mx * sl2 > thr), 0)) {
             mx = max_xor32(mx) * sl2;
             const bool move = mx > thr;
-            const float to = move ? mx - kBias : ref;
+            // (a little further for scores whose last bit is more than 1: p has to stay below 2^16)
+            const float to = move ? mx - kBias + fabsf(mx) * 0x1p-22f : ref;
             const float corr = thr > -FLT_MAX ? fast_exp2(ref - to) : 1.f;
             ref = to;
             thr = move ? mx + kLag : thr;
@@ -286,11 +318,11 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
             }
     };
 
-    store(lds.k[0], lds.v[0], nfull == 0);
+    store(0, 0, nfull == 0);
     issue(1);
     __syncthreads();
     f32x16 S = scores(lds.k[0], 0);
-    settle(S, j0 + set_at(0) * kSetKeys + ks * KT, std::true_type{});
+    settle(S, lds.kf[0] + ks * KT, j0 + set_at(0) * kSetKeys + ks * KT, std::true_type{});
     // (the wave that has products to issue goes first: the two waves of a SIMD then take turns with
     // products and settling; 4 x 700 tokens with cap and window 60.6 -> 57.2 us, 2000 behind 6000 1%)
     // One set, whose first scores are there: the next one from its registers into LDS, the one after
@@ -298,10 +330,10 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     int v3 = 0;  // the V buffer of the set
     auto set = [&](int i, auto masked_tag) {
         const char* kd = lds.k[i & 1];
-        char* kn = lds.k[(i + 1) & 1];
         const char* vd = lds.v[v3];
+        const float* kf = lds.kf[v3] + ks * KT;
         v3 = v3 == 2 ? 0 : v3 + 1;
-        store(kn, lds.v[v3], decltype(masked_tag)::value);
+        store((i + 1) & 1, v3, decltype(masked_tag)::value);
         if (!WIDE && ((i + 2) & (kWave - 1)) == 0) load_ids(i + 2);
         issue(i + 2);  // (sets past the last read nothing: zero-size descriptors)
         const int t0 = j0 + set_at(i) * kSetKeys + ks * KT;
@@ -311,15 +343,15 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
             f32x16 next = scores(kd, n + 1);
             weigh(S, vd, n);
             __builtin_amdgcn_s_setprio(0);
-            settle(next, t0 + 32 * (n + 1), masked_tag);
+            settle(next, kf + 32 * (n + 1), t0 + 32 * (n + 1), masked_tag);
             S = next;
         }
         __syncthreads();
         __builtin_amdgcn_s_setprio(1);
-        f32x16 next = scores(kn, 0);  // (past the last set: rows that were stored as zero, masked)
+        f32x16 next = scores(lds.k[(i + 1) & 1], 0);  // (past the last set: rows stored as zero, masked)
         weigh(S, vd, NS - 1);
         __builtin_amdgcn_s_setprio(0);
-        settle(next, j0 + set_at(i + 1) * kSetKeys + ks * KT, masked_tag);
+        settle(next, lds.kf[v3] + ks * KT, j0 + set_at(i + 1) * kSetKeys + ks * KT, masked_tag);
         S = next;
     };
     // sets whose next one is seen whole as well, then the rest (loops of their own: one loop with both

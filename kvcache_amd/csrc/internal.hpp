@@ -234,6 +234,8 @@ struct Tuning {
                                 // attended while the kernel plans the others (0: none)
     int chain_spin = 1 << 20;   // layer chain (kvc_rows_chain): polls before a grid-barrier wait gives
                                 // up and reports kDevErrBarrier (about a second at the default)
+    int chunk_tiles = -1;       // chunk attention plans: tiles for sequences of many rows: -1 by the batch's
+                                // work, 0 never, 1 always
 };
 // Dynamic LDS that caps decode workgroups per CU at wg_per_cu (0: none).
 size_t occupancy_lds(size_t static_lds, int wg_per_cu);

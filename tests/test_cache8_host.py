@@ -1,9 +1,12 @@
 """The operators around an 8-bit paged cache without a GPU: their refusals (validation precedes
 any HIP call), the plan of a ragged batch, and the plain forms the GPU tests compare with."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 from _cache8 import E4M3, chunk_attention, norm_rope, quantise, round_e4m3, values
+from _helpers import tuning
 from kvcache_amd import _native as N
 from kvcache_amd import ops
 
@@ -118,7 +121,8 @@ def test_plan_refuses():
 @pytest.mark.parametrize("Hq,Hkv,D,block", [(14, 2, 64, 16), (8, 8, 64, 16), (32, 8, 128, 16), (64, 2, 128, 32),
                                             (40, 1, 128, 16), (4, 2, 32, 16), (6, 3, 64, 10), (16, 2, 256, 64)])
 @pytest.mark.parametrize("window", [0, 1, 100, 1000])
-def test_plan_covers_every_row_and_key_once(Hq, Hkv, D, block, window):
+@pytest.mark.parametrize("tiles", [-1, 0, 1])
+def test_plan_covers_every_row_and_key_once(Hq, Hkv, D, block, window, tiles):
     """Every (row, head) lies in units whose key ranges are disjoint and hold every key it sees;
     partial rows are disjoint and within n_records; ranges begin at whole 16-row subtiles."""
     rng = np.random.default_rng(Hq + window)
@@ -127,7 +131,9 @@ def test_plan_covers_every_row_and_key_once(Hq, Hkv, D, block, window):
         ql = rng.integers(0 if n > 1 else 1, qmax + 1, n)
         tl = ql + rng.integers(0, tmax, n)
         off = np.concatenate([[0], np.cumsum(-(-tl // block))]) + 5
-        work, nu, nt, (nr, nw) = ops.chunk_plan(ql, tl, Hq, Hkv, D, block, window=window, tab_off=off)
+        with tuning("chunk_tiles", tiles):
+            work, nu, nt, (nr, nw) = ops.chunk_plan(ql, tl, Hq, Hkv, D, block, window=window, tab_off=off)
+        assert (tiles != 0 or nt == 0) and (tiles != 1 or qmax <= 16 or D not in (64, 128) or block % 16 or nt > 0)
         assert work.shape == (nu, 16) and work[0, 0] == nu and work[0, 1] == nt and work[0, 2] == nr
         start = np.concatenate([[0], np.cumsum(ql)])
         covered = np.zeros((int(ql.sum()), group), np.int64)
@@ -164,6 +170,14 @@ def test_plan_covers_every_row_and_key_once(Hq, Hkv, D, block, window):
             s = int(np.searchsorted(start, row, side="right") - 1)
             assert ranges[-1][1] == tl[s] - ql[s] + row - start[s] + tok
         assert (covered > 0).all()
+
+
+def test_tile_knob():
+    L = N.lib()
+    v = C.c_int(7)
+    assert L.kvc_get_tuning(b"chunk_tiles", C.byref(v)) == N.KVC_OK and v.value == -1
+    for bad in (-2, 2):
+        assert L.kvc_set_tuning(b"chunk_tiles", bad) == N.KVC_ERR_ARG
 
 
 def test_plan_of_an_empty_batch():

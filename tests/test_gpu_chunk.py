@@ -6,13 +6,20 @@ import numpy as np
 import pytest
 
 from _cache8 import (NAME, chunk_attention, chunk_bound, code_dtype, norm_rope, quantise, values)
-from _helpers import dev, host, say
+from _helpers import dev, host, say, tuning
 from kvcache_amd import KVC_E4M3, KVC_F16, KVC_I8, ops
 from kvcache_amd._native import check, lib
 from kvcache_amd.device import DeviceBuffer, Stream, synchronize
 
 pytestmark = pytest.mark.gpu
 ALL = [KVC_F16, KVC_I8, KVC_E4M3]
+
+
+@pytest.fixture(params=[-1, 1], ids=["auto", "tiles"], autouse=True)
+def tiles(request):
+    """Batches this small go to units of 16 rows by themselves; each test runs with tiles as well."""
+    with tuning("chunk_tiles", request.param):
+        yield request.param
 
 
 class Batch:
@@ -140,6 +147,24 @@ def test_large_scores_and_values_of_many_sizes(D, kv):
     Batch([80, 1], [333, 900], 8, 2, D, 16, kv, seed=4, spread=2.0, k_std=0.3).check()
     Batch([80, 1], [333, 900], 8, 2, D, 16, kv, seed=5).check(scale=-0.1)
     Batch([80, 1], [333, 900], 8, 2, D, 16, kv, seed=6).check(scale=0.0)
+    Batch([80, 1], [333, 900], 8, 2, D, 16, kv, seed=7, spread=0.1, k_std=9000.0).check(scale=40.0)  # (K up to 6e4)
+    Batch([80, 1], [333, 900], 8, 2, D, 16, kv, seed=8, k_std=1e-4).check(scale=1000.0)
+
+
+@pytest.mark.parametrize("kv", ALL, ids=NAME.get)
+@pytest.mark.parametrize("D,hq,hkv", [(64, 14, 2), (128, 8, 2), (128, 2, 2)])
+def test_many_rows_over_split_keys(D, hq, hkv, kv, tiles):
+    """Few tiles over many keys: their key ranges are split and merged, with whole tiles beside them;
+    a window that leaves chunks of some rows empty; a first token that sees a single key."""
+    b = Batch([140, 66, 3], [5000, 66, 3000], hq, hkv, D, 16, kv, seed=60)
+    a = b.check()
+    work, nu, nt, (nr, nw) = b.plan
+    if tiles == 1:
+        assert nt > 0 and nr > 0 and (kv == KVC_F16) == (nw == 0)
+        kinds = np.asarray(work).reshape(-1, 16)[1:]
+        assert len(kinds) == nu - 1
+    assert (b.run() == a).all()
+    Batch([140, 66, 3], [5000, 66, 3000], hq, hkv, D, 16, kv, seed=61).check(window=2100, cap=20.0)
 
 
 @pytest.mark.parametrize("kv", ALL, ids=NAME.get)
