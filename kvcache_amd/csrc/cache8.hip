@@ -35,14 +35,14 @@ struct RopeWriteParams {
     int M, Hq, Hkv, block, tokens;  // tokens: per workgroup
 };
 
-// The two vectors of a lane into a pool row (16 or 8 bytes each) and its scale.
+// The two vectors of a lane into a pool row (16 or 8 bytes each); the row's scale.
 template <int D, int CT>
-__device__ __forceinline__ void store_row(void* pool, float* scales, int which, size_t row, int l, const float (&a)[8],
-                                          const float (&b)[8], bool first) {
+__device__ __forceinline__ float store_row(void* pool, size_t row, int l, const float (&a)[8], const float (&b)[8]) {
     if constexpr (CT == kCacheF16) {
         _Float16* o = static_cast<_Float16*>(pool) + row * D + 8 * l;
         *reinterpret_cast<u32x4*>(o) = Traits<_Float16>::from_float(a);
         *reinterpret_cast<u32x4*>(o + D / 2) = Traits<_Float16>::from_float(b);
+        return 1.f;
     } else {
         unsigned mx = 0;
 #pragma unroll
@@ -53,7 +53,7 @@ __device__ __forceinline__ void store_row(void* pool, float* scales, int which, 
         unsigned char* o = static_cast<unsigned char*>(pool) + row * D + 8 * l;
         *reinterpret_cast<u32x2*>(o) = values_to_codes<CT>(a, inv);
         *reinterpret_cast<u32x2*>(o + D / 2) = values_to_codes<CT>(b, inv);
-        if (first) scales[row * 2 + which] = s;
+        return s;
     }
 }
 
@@ -118,7 +118,8 @@ __global__ __launch_bounds__(kRowThreads) void norm_rope_write_kernel(RopeWriteP
             const int hk = h - p.Hq - (is_v ? p.Hkv : 0);
             const int blk = slot / p.block;
             const size_t row = ((size_t)blk * p.Hkv + hk) * p.block + (slot - blk * p.block);
-            store_row<D, CT>(is_v ? p.v_pool : p.k_pool, p.scales, is_v, row, l, a, b, l == 0);
+            const float s = store_row<D, CT>(is_v ? p.v_pool : p.k_pool, row, l, a, b);
+            if (CT != kCacheF16 && l == 0) p.scales[row * 2 + is_v] = s;
         }
     }
 }
@@ -156,51 +157,63 @@ __device__ __forceinline__ void store8(void* base, size_t at, const float (&f)[8
     }
 }
 
+// A workgroup: kRowThreads / LPR consecutive tokens of one head, K and V of a token in one thread (the
+// rows of a block and its scales then leave as whole lines).  40009 tokens of 8 heads, D 128, int8,
+// written and read back, 497 MB: 105 us, of 99 at the rate of a large copy; one row of K or V per
+// thread, head after head, 121 us (scales in lines that several XCDs write).
+template <int LPR>
+__device__ __forceinline__ bool row_of(const RowsParams& p, int& r, int& hk, int& l) {
+    const unsigned chunk = blockIdx.x / (unsigned)p.Hkv;
+    hk = (int)(blockIdx.x - chunk * (unsigned)p.Hkv);
+    r = (int)(chunk * (kRowThreads / LPR) + threadIdx.x / LPR);
+    l = threadIdx.x % LPR;
+    return r < p.rows;
+}
+__device__ __forceinline__ size_t pool_row(const RowsParams& p, int slot, int hk) {
+    const int blk = slot / p.block;
+    return ((size_t)blk * p.Hkv + hk) * p.block + (slot - blk * p.block);
+}
+
 template <typename T, int D, int CT>
 __global__ __launch_bounds__(kRowThreads) void write_q8_kernel(RowsParams p) {
-    constexpr int LPR = D / 16;
-    const long long it = ((long long)blockIdx.x * kRowThreads + threadIdx.x) / LPR;  // (row, k or v, head)
-    if (it >= (long long)p.rows * 2 * p.Hkv) return;
-    const int l = threadIdx.x % LPR;
-    const int r = (int)(it / (2 * p.Hkv)), h = (int)(it - (long long)r * 2 * p.Hkv);
+    int r, hk, l;
+    if (!row_of<D / 16>(p, r, hk, l)) return;
     const int slot = p.slots[r];
-    if (slot < 0) return;
-    const bool is_v = h >= p.Hkv;
-    const int hk = is_v ? h - p.Hkv : h;
     const size_t src = ((size_t)r * p.Hkv + hk) * D + 8 * l;
-    float a[8], b[8];
-    load8<T>(is_v ? p.v : p.k, src, a);
-    load8<T>(is_v ? p.v : p.k, src + D / 2, b);
-    const int blk = slot / p.block;
-    const size_t row = ((size_t)blk * p.Hkv + hk) * p.block + (slot - blk * p.block);
-    store_row<D, CT>(is_v ? p.v_pool : p.k_pool, p.scales, is_v, row, l, a, b, l == 0);
+    float k0[8], k1[8], v0[8], v1[8];
+    load8<T>(p.k, src, k0);
+    load8<T>(p.k, src + D / 2, k1);
+    load8<T>(p.v, src, v0);
+    load8<T>(p.v, src + D / 2, v1);
+    if (slot < 0) return;
+    const size_t row = pool_row(p, slot, hk);
+    f32x2 s;
+    s[0] = store_row<D, CT>(p.k_pool, row, l, k0, k1);
+    s[1] = store_row<D, CT>(p.v_pool, row, l, v0, v1);
+    if (l == 0) *reinterpret_cast<f32x2*>(p.scales + row * 2) = s;
 }
 
 template <typename T, int D, int CT>
 __global__ __launch_bounds__(kRowThreads) void read_kernel(RowsParams p, void* k_out, void* v_out) {
-    constexpr int LPR = D / 8;
-    const long long it = ((long long)blockIdx.x * kRowThreads + threadIdx.x) / LPR;
-    if (it >= (long long)p.rows * 2 * p.Hkv) return;
-    const int l = threadIdx.x % LPR;
-    const int r = (int)(it / (2 * p.Hkv)), h = (int)(it - (long long)r * 2 * p.Hkv);
+    int r, hk, l;
+    if (!row_of<D / 8>(p, r, hk, l)) return;
     const int slot = p.slots[r];
     if (slot < 0) return;
-    const bool is_v = h >= p.Hkv;
-    const int hk = is_v ? h - p.Hkv : h;
-    const int blk = slot / p.block;
-    const size_t row = ((size_t)blk * p.Hkv + hk) * p.block + (slot - blk * p.block);
-    const void* pool = is_v ? p.v_pool : p.k_pool;
-    float a[8];
+    const size_t row = pool_row(p, slot, hk), from = row * D + 8 * l, to = ((size_t)r * p.Hkv + hk) * D + 8 * l;
+    float a[8], b[8];
     if constexpr (CT == kCacheF16) {
-        load8<_Float16>(pool, row * D + 8 * l, a);
+        load8<_Float16>(p.k_pool, from, a);
+        load8<_Float16>(p.v_pool, from, b);
     } else {
-        const u32x2 c = *reinterpret_cast<const u32x2*>(static_cast<const unsigned char*>(pool) + row * D + 8 * l);
-        const f16x8 x = codes_to_f16x8<CT>(c);
-        const float s = p.scales[row * 2 + is_v];
+        const u32x2 ck = *reinterpret_cast<const u32x2*>(static_cast<const unsigned char*>(p.k_pool) + from);
+        const u32x2 cv = *reinterpret_cast<const u32x2*>(static_cast<const unsigned char*>(p.v_pool) + from);
+        const f32x2 s = *reinterpret_cast<const f32x2*>(p.scales + row * 2);
+        const f16x8 x = codes_to_f16x8<CT>(ck), y = codes_to_f16x8<CT>(cv);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] = (float)x[e] * s;
+        for (int e = 0; e < 8; ++e) a[e] = (float)x[e] * s[0], b[e] = (float)y[e] * s[1];
     }
-    store8<T>(is_v ? v_out : k_out, ((size_t)r * p.Hkv + hk) * D + 8 * l, a);
+    store8<T>(k_out, to, a);
+    store8<T>(v_out, to, b);
 }
 
 template <typename F>
@@ -221,6 +234,11 @@ int guard_rows(F&& f) {
     } catch (...) {
         return set_error(KVC_ERR_STATE, "unexpected exception");
     }
+}
+
+unsigned row_groups(int rows, int Hkv, int lanes) {
+    const int per = kRowThreads / lanes;
+    return (unsigned)((rows + (long long)per - 1) / per * Hkv);
 }
 
 bool a16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
@@ -300,8 +318,7 @@ int kvc_write_kv_q8(const void* k, const void* v, void* k_pool, void* v_pool, fl
         const RowsParams p{k, v, k_pool, v_pool, kv_scales, slot_map, rows, Hkv, BLOCK};
         return for_head_dim(D, [&](auto d) -> int {
             constexpr int kD = decltype(d)::value;
-            const long long lanes = (long long)rows * 2 * Hkv * (kD / 16);
-            const dim3 grid((unsigned)((lanes + kRowThreads - 1) / kRowThreads)), block(kRowThreads);
+            const dim3 grid(row_groups(rows, Hkv, kD / 16)), block(kRowThreads);
             const hipStream_t s = (hipStream_t)st;
             if (dtype == KVC_F16 && kv_dtype == KVC_I8)
                 hipLaunchKernelGGL((write_q8_kernel<_Float16, kD, kCacheI8>), grid, block, 0, s, p);
@@ -328,8 +345,7 @@ int kvc_read_kv(void* k, void* v, const void* k_pool, const void* v_pool, const 
                            const_cast<float*>(kv_scales), slot_map, rows, Hkv, BLOCK};
         return for_head_dim(D, [&](auto d) -> int {
             constexpr int kD = decltype(d)::value;
-            const long long lanes = (long long)rows * 2 * Hkv * (kD / 8);
-            const dim3 grid((unsigned)((lanes + kRowThreads - 1) / kRowThreads)), block(kRowThreads);
+            const dim3 grid(row_groups(rows, Hkv, kD / 8)), block(kRowThreads);
             const hipStream_t s = (hipStream_t)st;
             auto launch = [&](auto ct) {
                 constexpr int kCT = decltype(ct)::value;
