@@ -198,12 +198,7 @@ Plan plan_batched(int N, int Hq, int Hkv, int D, int BLOCK, int cap, int dtype, 
     return pl;
 }
 
-// Call tag for the fused-merge arrival counters; never 0 (0 is the reset value).
 std::atomic<unsigned> g_epoch{0x9e3779b9u};
-unsigned next_epoch() {
-    unsigned e = g_epoch.fetch_add(1u, std::memory_order_relaxed) + 1u;
-    return e ? e : g_epoch.fetch_add(1u, std::memory_order_relaxed) + 1u;
-}
 
 // Library-owned grow-only workspace per (device, stream), used when the caller passes
 // none.  Launches on one stream run in order, so they can share a buffer; launches on
@@ -260,6 +255,12 @@ std::mutex g_err_mu;
 std::vector<int*> g_err_words;
 
 }  // namespace
+
+// Call tag for the fused-merge arrival counters; never 0 (0 is the reset value).
+unsigned next_epoch() {
+    unsigned e = g_epoch.fetch_add(1u, std::memory_order_relaxed) + 1u;
+    return e ? e : g_epoch.fetch_add(1u, std::memory_order_relaxed) + 1u;
+}
 
 int library_workspace(size_t bytes, hipStream_t st, void** out) { return default_workspace(bytes, st, out); }
 

@@ -15,6 +15,7 @@ size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 size_t acc_bytes(int Hkv, int D, int n_records) { return up((size_t)Hkv * n_records * D * sizeof(float), kPartAlign); }
 size_t wide_bytes(int Hkv, int D, int n_wide) { return up((size_t)Hkv * n_wide * D * 2, kPartAlign); }
 size_t ml_bytes(int Hkv, int n_records) { return up((size_t)Hkv * n_records * 2 * sizeof(float), kPartAlign); }
+size_t ctr_bytes(int Hkv, int n_records) { return up((size_t)Hkv * n_records * sizeof(unsigned long long), kPartAlign); }
 size_t factor_bytes(int Hkv, int n_wide) { return up((size_t)Hkv * n_wide * sizeof(float), kPartAlign); }
 
 int check_shape(int Hq, int Hkv, int D, int BLOCK, int kv_dtype, int window) {
@@ -243,10 +244,13 @@ int launch_chunks_d(const ChunkParams& p, int n_tiles, hipStream_t st) {
     if (!matrix) hipLaunchKernelGGL((chunk_rows_kernel<D, CT>), dim3(units * Hkv), dim3(256), 0, st, p);
     int rc = hip_check(hipGetLastError(), "chunk attention launch");
     if (rc || p.n_records == 0) return rc;
+    const unsigned split = matrix ? tiles : units;  // (units of 16 rows combine their own)
+    if (split == 0) return KVC_OK;
     // a workgroup's share of the rows in about one pass
-    const long long passes = ((long long)p.n_records * (D / 4) + 256LL * units - 1) / (256LL * units);
-    hipLaunchKernelGGL((merge_chunks_kernel<D>), dim3(units * Hkv, (unsigned)std::min(8LL, std::max(1LL, passes))), dim3(256),
-                       0, st, p);
+    const long long passes = ((long long)p.n_records * (D / 4) + 256LL * split - 1) / (256LL * split);
+    const dim3 grid(split * Hkv, (unsigned)std::min(8LL, std::max(1LL, passes)));
+    if (matrix) hipLaunchKernelGGL((merge_chunks_kernel<D, true>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((merge_chunks_kernel<D, false>), grid, dim3(256), 0, st, p);
     return hip_check(hipGetLastError(), "chunk attention merge launch");
 }
 
@@ -306,7 +310,7 @@ size_t kvc_chunk_workspace_size(int Hq, int Hkv, int D, int n_records, int n_wid
     if (Hq <= 0 || Hkv <= 0 || D <= 0) return 0;
     n_records = std::max(n_records, 0);
     n_wide = std::max(n_wide, 0);
-    return acc_bytes(Hkv, D, n_records) + ml_bytes(Hkv, n_records) + 2 * wide_bytes(Hkv, D, n_wide) + factor_bytes(Hkv, n_wide);
+    return acc_bytes(Hkv, D, n_records) + ml_bytes(Hkv, n_records) + ctr_bytes(Hkv, n_records) + 2 * wide_bytes(Hkv, D, n_wide) + factor_bytes(Hkv, n_wide);
 }
 
 int kvc_paged_chunk_attn(const void* q, void* out, const void* k_pool, const void* v_pool, const float* kv_scales,
@@ -358,6 +362,9 @@ int kvc_paged_chunk_attn(const void* q, void* out, const void* k_pool, const voi
             ws += acc_bytes(Hkv, D, n_records);
             p.part_ml = reinterpret_cast<float*>(ws);
             ws += ml_bytes(Hkv, n_records);
+            p.counters = reinterpret_cast<unsigned long long*>(ws);
+            p.epoch = next_epoch();
+            ws += ctr_bytes(Hkv, n_records);
             p.wide_k = reinterpret_cast<_Float16*>(ws);
             ws += wide_bytes(Hkv, D, n_wide);
             p.wide_v = reinterpret_cast<_Float16*>(ws);

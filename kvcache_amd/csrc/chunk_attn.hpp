@@ -5,7 +5,8 @@
 // consecutive tokens of one sequence times hn query heads of each KV head, over keys j0 .. j1-1;
 // a workgroup takes one unit of one KV head.  Its rows r = (token i, head g) = (r / hn, r % hn)
 // share every K and V row it reads.  A unit whose key range is one of nc > 1 leaves partial rows
-// (running maximum in log2 units, sum, unnormalised output) that merge_chunks combines.
+// (running maximum in log2 units, sum, unnormalised output): of the units of 16 rows on the matrix
+// cores the last one to arrive combines them, of the others merge_chunks_kernel does.
 #pragma once
 #include "cache8.hpp"
 
@@ -26,6 +27,7 @@ struct ChunkParams {
     int n_wide;             // ... and widened keys
     int rows, Hq, Hkv, group, block;
     int table_len, window;
+    unsigned epoch;         // the launch's tag of its arrival counters
     float scale_log2;       // softmax scale * log2(e)
     float cap_log2;         // softcap * log2(e), 0: none
     float cap_in;           // score -> argument of the cap's exponential: 2 * scale * log2(e) / softcap
@@ -37,6 +39,7 @@ struct ChunkParams {
     const int* table;
     float* part_acc;        // [Hkv][n_records][D]
     float* part_ml;         // [Hkv][n_records][2]
+    unsigned long long* counters;  // [Hkv][n_records]: arrivals of the units whose records begin there
     _Float16* wide_k;       // [Hkv][n_wide][D]
     _Float16* wide_v;
     float* wide_f;          // [Hkv][n_wide]: the score's factor
@@ -251,6 +254,65 @@ __device__ __forceinline__ f32x4 add_seen_nonfinite(const ChunkParams& p, const 
     }
     return acc;
 }
+
+// Partials that another workgroup of the launch reads: 16 bytes past the caches that are not
+// coherent between XCDs, to the device's point of coherence (sc1, what agent-scope accesses use).
+constexpr int kCoherent = 16;
+__device__ __forceinline__ void store_coherent(__amdgpu_buffer_rsrc_t r, int at, f32x4 x) {
+    typedef int v4i __attribute__((ext_vector_type(4)));
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, x), r, at, 0, kCoherent);
+}
+__device__ __forceinline__ f32x4 load_coherent(__amdgpu_buffer_rsrc_t r, int at) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, kCoherent));
+}
+__device__ __forceinline__ void store_coherent2(__amdgpu_buffer_rsrc_t r, int at, f32x2 x) {
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2i, x), r, at, 0, kCoherent);
+}
+__device__ __forceinline__ f32x2 load_coherent2(__amdgpu_buffer_rsrc_t r, int at) {
+    return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, kCoherent));
+}
+
+// Running (M, l, acc) of four dims of a row over chunks c0, c0 + step, .. of its nc, eight in flight;
+// at(c): a chunk's record, as (m, l) and the four dims.
+struct MergedRow {
+    float M = -FLT_MAX, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    template <typename F>
+    __device__ __forceinline__ void add(int c0, int step, int nc, F&& at) {
+        constexpr int E = 8;
+        for (; c0 < nc; c0 += E * step) {
+            // (past the count the last chunk's again, with weight 0)
+            f32x2 ml[E];
+            f32x4 a[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) at(min(c0 + e * step, nc - 1), ml[e], a[e]);
+            float top = M;
+#pragma unroll
+            for (int e = 0; e < E; ++e) top = fmaxf(top, ml[e][0]);
+            const float w0 = fast_exp2(M - top);
+            M = top;
+            l *= w0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[k] *= w0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (c0 + e * step >= nc) continue;
+                const float w = fast_exp2(ml[e][0] - M);
+                l = __builtin_fmaf(w, ml[e][1], l);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] = __builtin_fmaf(w, a[e][k], acc[k]);
+            }
+        }
+    }
+    __device__ __forceinline__ f16x4 out() const {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        f16x4 o;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = (_Float16)(acc[k] * inv);
+        return o;
+    }
+};
 
 template <int D, int CT, int R>
 __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUnit& u, char* lds) {
@@ -549,6 +611,10 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
 #pragma unroll
         for (int w = 0; w < W; ++w) any_bad |= s_bad[w];
     }
+    // (nc rows * D floats: below 2^31 bytes in every plan; what a list of other counts reaches is in bounds)
+    const size_t first = (size_t)u.hk * p.n_records + u.rec0;
+    const int recs = u.nc == 1 ? 0 : min(u.nc, (1 << 20) / u.rows) * u.rows;
+    const __amdgpu_buffer_rsrc_t ar = tile_rsrc(p.part_acc + first * D, recs * D * 4), mr = tile_rsrc(p.part_ml + first * 2, recs * 8);
     for (int idx = threadIdx.x; idx < u.rows * (D / 4); idx += W * kWave) {
         const int r = idx / (D / 4), d = idx % (D / 4) * 4;
         float M = -FLT_MAX;
@@ -570,14 +636,56 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
             for (int e = 0; e < 4; ++e) o[e] = (_Float16)(at[e] * inv);
             *reinterpret_cast<f16x4*>(p.out + chunk_row(p, u, r, D) + d) = o;
         } else {
-            const size_t rec = (size_t)u.hk * p.n_records + u.rec0 + (size_t)u.c * u.rows + r;
-            *reinterpret_cast<f32x4*>(p.part_acc + rec * D + d) = at;
-            if (d == 0) {
-                p.part_ml[rec * 2] = M;
-                p.part_ml[rec * 2 + 1] = lt;
-            }
+            const int rec = u.c * u.rows + r;
+            store_coherent(ar, (rec * D + d) * 4, at);
+            if (d == 0) store_coherent2(mr, rec * 8, f32x2{M, lt});
         }
     }
+    if (u.nc == 1) return;
+
+    // The last of the nc units to arrive combines their partials, always in the order of the chunks.
+    // Its threads are 16-byte pieces of the rows times as many groups of chunks as there is room for.
+    __shared__ int s_last;
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's partials are written
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    unsigned long long* ctr = p.counters + (size_t)u.hk * p.n_records + u.rec0;
+    if (threadIdx.x == 0) s_last = arrive(ctr, p.epoch) == (unsigned)(u.nc - 1);
+    __syncthreads();
+    if (!s_last) return;
+    constexpr int TD = D / 4, NTH = W * kWave;
+    const int items = u.rows * TD;
+    int groups = 1;
+    while (2 * groups * items <= NTH && 4 * groups < u.nc) groups *= 2;
+    f32x4* s_acc = reinterpret_cast<f32x4*>(lds);
+    f32x2* s_wl = reinterpret_cast<f32x2*>(lds + NTH * sizeof(f32x4));
+    static_assert(NTH * 24 <= Sh::kBytes, "the groups' sums fit the tiles");
+    for (int i0 = 0; i0 < items; i0 += NTH / groups) {
+        const int g = groups == 1 ? 0 : threadIdx.x / items, i = i0 + threadIdx.x - g * items;
+        const bool on = g < groups && i < items;
+        const int r = i / TD, d = i % TD * 4;
+        MergedRow x;
+        if (on)
+            x.add(g, groups, u.nc, [&](int c, f32x2& ml, f32x4& a) {
+                const int rec = c * u.rows + r;
+                ml = load_coherent2(mr, rec * 8);
+                a = load_coherent(ar, (rec * D + d) * 4);
+            });
+        if (groups > 1) {  // (then one pass covers every item)
+            s_acc[threadIdx.x] = x.acc;
+            s_wl[threadIdx.x] = f32x2{x.M, x.l};
+            __syncthreads();
+            x = MergedRow{};
+            if (g == 0)
+                x.add(0, 1, groups, [&](int c, f32x2& ml, f32x4& a) {
+                    ml = s_wl[c * items + threadIdx.x];
+                    a = s_acc[c * items + threadIdx.x];
+                });
+        }
+        if (on && g == 0) *reinterpret_cast<f16x4*>(p.out + chunk_row(p, u, r, D) + d) = x.out();
+    }
+    if (threadIdx.x == 0) __hip_atomic_store(ctr, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 template <int D, int CT>
@@ -589,50 +697,23 @@ __global__ __launch_bounds__(kStreamWaves * kWave, D == 64 ? 4 : 2) void chunk_s
 }
 
 // Partial rows of the units with nc > 1 as output rows: out = sum_c 2^(m_c - M) acc_c / sum_c
-// 2^(m_c - M) l_c.  A thread takes four dims of a row over all its chunks, eight of them in flight;
-// the workgroups of a tile's nc units (times gridDim.y) share its rows.
-template <int D>
+// 2^(m_c - M) l_c.  A thread takes four dims of a row over all its chunks; the workgroups of a tile's
+// nc units (times gridDim.y) share its rows.  TILES: of the tiles only.
+template <int D, bool TILES>
 __global__ __launch_bounds__(256) void merge_chunks_kernel(ChunkParams p) {
-    constexpr int TD = D / 4, E = 8;
+    constexpr int TD = D / 4;
     ChunkUnit u;
-    if (!chunk_unit(p, u, 0) || u.nc == 1) return;
+    if (!chunk_unit(p, u, 0) || u.nc == 1 || (TILES && u.kind != kKindTile)) return;
     const size_t head = (size_t)u.hk * p.n_records + u.rec0;
     for (int i = (blockIdx.y * u.nc + u.c) * 256 + threadIdx.x; i < u.rows * TD; i += gridDim.y * u.nc * 256) {
         const int r = i / TD, d = i % TD * 4;
-        float M = -FLT_MAX, l = 0.f;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int c0 = 0; c0 < u.nc; c0 += E) {
-            // (past the count the last chunk's again, with weight 0)
-            f32x2 ml[E];
-            f32x4 a[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const size_t rec = head + (size_t)min(c0 + e, u.nc - 1) * u.rows + r;
-                ml[e] = *reinterpret_cast<const f32x2*>(p.part_ml + rec * 2);
-                a[e] = *reinterpret_cast<const f32x4*>(p.part_acc + rec * D + d);
-            }
-            float top = M;
-#pragma unroll
-            for (int e = 0; e < E; ++e) top = fmaxf(top, ml[e][0]);
-            const float w0 = fast_exp2(M - top);
-            M = top;
-            l *= w0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[k] *= w0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if (c0 + e >= u.nc) continue;
-                const float w = fast_exp2(ml[e][0] - M);
-                l = __builtin_fmaf(w, ml[e][1], l);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[k] = __builtin_fmaf(w, a[e][k], acc[k]);
-            }
-        }
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-        f16x4 o;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = (_Float16)(acc[k] * inv);
-        *reinterpret_cast<f16x4*>(p.out + chunk_row(p, u, r, D) + d) = o;
+        MergedRow x;
+        x.add(0, 1, u.nc, [&](int c, f32x2& ml, f32x4& a) {
+            const size_t rec = head + (size_t)c * u.rows + r;
+            ml = *reinterpret_cast<const f32x2*>(p.part_ml + rec * 2);
+            a = *reinterpret_cast<const f32x4*>(p.part_acc + rec * D + d);
+        });
+        *reinterpret_cast<f16x4*>(p.out + chunk_row(p, u, r, D) + d) = x.out();
     }
 }
 

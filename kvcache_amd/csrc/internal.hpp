@@ -17,6 +17,9 @@ int hip_check(hipError_t e, const char* what);
 // KVC_ERR_STATE while the stream is capturing (abi.hip).
 int library_workspace(size_t bytes, hipStream_t st, void** out);
 
+// A launch's tag for its arrival counters (decode_kernels.hpp, arrive); never 0.
+unsigned next_epoch();
+
 // ---------------------------------------------------------------------------
 // Decode launch description (host side).  One "unit" = (sequence s, KV head hk,
 // query-head subgroup sub, chunk c); each unit is one workgroup of `wpb` waves.
