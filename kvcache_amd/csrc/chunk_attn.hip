@@ -47,10 +47,10 @@ struct PlanUnit {
 // Keys per chunk of the units of 16 rows, `keys` of them over all units and KV heads.  Two
 // workgroups fit a CU (512), and chunks of 512 keys keep them in flight; below that a batch is
 // still cut for one workgroup a CU down to 256 keys (one round of four waves).  int8, 32q/8kv, D
-// 128: one sequence of 4000 38.4 us whole, 15.2 in chunks of 1024, 9.1 in 256; 64 of 32..4096 43.4
+// 128: one sequence of 4000 38.4 us whole, 15.2 in chunks of 1024, 10.4 in 256; 64 of 32..4096 43.4
 // whole, 34.6 for 256 workgroups, 30.8 for 512; 16 of 4000 (8q/8kv, D 64) 33 whole, 24.1 and 22.9.
-// At most 32 chunks of a sequence, whose merge grows with them (one of 20000, 8q/8kv: 14.1 us in 40
-// chunks, 13.4 in 32, 17.5 in 63).
+// At most 32 chunks of a sequence, whose arrivals are served one after the other (one of 20000,
+// 8q/8kv: 13.3 us in 32 chunks, 17.8 in 40, 19.8 in 63).
 long long stream_chunk(long long keys, int longest) {
     const long long one = (keys + 255) / 256, two = (keys + 511) / 512;
     const long long c = std::max(256LL, std::min(one, std::max(two, 512LL)));
@@ -64,7 +64,9 @@ int chunks_of(long long len, long long c) { return len > c * 3 / 2 ? (int)((len 
 // for one, two or three rounds of the card's workgroups.  A set of 64 keys takes a tile of 256 rows
 // 2.1 us at head_dim 128 (one workgroup a CU), 1.8 at 64 (two a CU), a unit another 4; the partials
 // are written and read at about 4 TB/s and merged by a launch of 4 us.  2000 tokens of 32 heads
-// behind 4000, D 128 (256 workgroups whole): 103 us whole, 125 in 320 workgroups.
+// behind 4000, D 128 (256 workgroups whole): 103 us whole, 125 in 320 workgroups.  At least 512 keys
+// (D 128: 256): 700 behind 3000, 14q/2kv, D 64, int8, 34 us in chunks of 512, 39 of 256; 400 behind
+// 1000, 32q/8kv, D 128, 37.5 and 35.6.
 long long tile_chunk(const std::vector<Tile>& tiles, int Hkv, int D) {
     long long keys = 0, longest = 0, rows_keys = 0, n = 0;
     for (const Tile& t : tiles) {
@@ -98,7 +100,7 @@ long long tile_chunk(const std::vector<Tile>& tiles, int Hkv, int D) {
     long long best = INT_MAX;
     double least = estimate(INT_MAX / 2);
     for (int k = 1; k <= 3; ++k) {
-        long long c = std::max(512LL, (keys * Hkv + k * slots - 1) / (k * slots));
+        long long c = std::max(D == 128 ? 256LL : 512LL, (keys * Hkv + k * slots - 1) / (k * slots));
         for (int i = 0; i < 40 && c < longest && units(c) > k * slots; ++i) c += c / 16 + 1;
         c = (c + 63) / 64 * 64;
         if (c >= longest) continue;
@@ -115,11 +117,12 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
                 int kv_dtype, int window, std::vector<PlanUnit>& units, long long& records, long long& wide) {
     const int group = Hq / Hkv;
     auto first_key = [&](int pos) { return window > 0 ? std::max(0, pos - window + 1) / 64 * 64 : 0; };
-    // Tiles reach about three times the rate of units of 16 rows, but take a launch more, 8-bit caches
-    // two (widening).  One sequence, int8 (fp16), units of 16 and tiles: 14q/2kv, D 64, 400 tokens
-    // behind 1000 (1.7 GFLOP) 17 and 19 us (15 and 16), 1000 behind 1000 (5.4) 30 and 30 (26 and 25),
-    // 400 behind 4000 (6.0) 36 and 31 (32 and 25); 32q/8kv, D 128, 64 behind 4000 (4.2) 24 and 27 (23
-    // and 19), 400 behind 1000 (7.9) 38 and 35 (37 and 30), 150 behind 4000 (10) 50 and 39 (48 and 31).
+    // Tiles reach about three times the rate of units of 16 rows, but take a launch or two more (merge;
+    // 8-bit caches: widening).  One sequence, int8 (fp16), units of 16 and tiles: 14q/2kv, D 64, 400
+    // tokens behind 1000 (1.7 GFLOP) 17 and 25 us (15 and 20), 1000 behind 1000 (5.4) 28 and 30 (25 and
+    // 24), 400 behind 4000 (6.0) 41 and 31 (36 and 24); 32q/8kv, D 128, 64 behind 4000 (4.2) 23 and 33
+    // (23 and 25), 500 behind 500 (6.1) 30 and 33 (28 and 27), 400 behind 1000 (7.9) 38 and 36 (36 and
+    // 28), 150 behind 4000 (10) 50 and 40 (49 and 31).
     bool tiled = false;
     if (matrix_path(D, BLOCK)) {
         double flops = 0;
@@ -129,7 +132,7 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
                 flops += 4.0 * D * Hq * n * (window > 0 ? std::min<double>(seen, window) : seen);
             }
         const int knob = tuning().chunk_tiles;
-        tiled = knob >= 0 ? knob == 1 : flops >= (D == 64 ? 5e9 : 7e9) * (kv_dtype == KVC_F16 ? 0.6 : 1.0);
+        tiled = knob >= 0 ? knob == 1 : flops >= (D == 64 ? 5.6e9 : 7e9) * (kv_dtype == KVC_F16 ? 0.6 : 1.0);
     }
     std::vector<Tile> tiles;
     long long row = 0, tab = 0, stream_keys = 0;
