@@ -404,7 +404,9 @@ int kvc_read_kv(void* k, void* v, const void* k_pool, const void* v_pool, const 
  * p = kv_lens[s] - q_lens[s] + i and attends to keys max(0, p - window + 1) .. p (window 0: from
  * 0); scores are scale * q.k, with softcap > 0 softcap * tanh(score / softcap).  q and out are
  * [rows, Hq, D] fp16, the sequences' tokens one after the other; statistics are fp32.  A row
- * whose scores are all -Inf gets zeros; NaN and Inf in K or V reach the rows that see their key.
+ * whose scores are all -Inf gets zeros; NaN and Inf in K or V reach the rows that see their key
+ * (an e4m3 code of NaN, which no call here writes, may reach any row of its sequence).  q and
+ * out may be one buffer.
  *
  * K and V values of up to 65504 in size (fp16's range) count as what they are, larger ones may
  * count as Inf.

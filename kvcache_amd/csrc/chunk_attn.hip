@@ -284,6 +284,8 @@ int kvc_chunk_plan(const int* host_q_lens, const int* host_kv_lens, const int* h
             if (host_q_lens[s] < 0 || host_kv_lens[s] < host_q_lens[s])
                 return set_error(KVC_ERR_ARG, "sequence " + std::to_string(s) + ": 0 <= q_lens <= kv_lens is needed");
             if (host_tab_off && host_tab_off[s] < 0) return set_error(KVC_ERR_ARG, "negative table offset");
+            if (host_tab_off && host_tab_off[s] + ((long long)host_kv_lens[s] + BLOCK - 1) / BLOCK > INT_MAX)
+                return set_error(KVC_ERR_UNSUPPORTED, "at most 2^31 - 1 rows and table entries");
             rows += host_q_lens[s];
             blocks += ((long long)host_kv_lens[s] + BLOCK - 1) / BLOCK;
         }
@@ -344,6 +346,8 @@ int kvc_paged_chunk_attn(const void* q, void* out, const void* k_pool, const voi
         p.scale_log2 = scale * log2e;
         p.cap_log2 = softcap * log2e;
         p.cap_in = softcap > 0.f ? 2.f * scale * log2e / softcap : 0.f;
+        if (!std::isfinite(p.scale_log2) || !std::isfinite(p.cap_log2) || !std::isfinite(p.cap_in))
+            return set_error(KVC_ERR_ARG, "scale, softcap and scale / softcap must be within fp32's range in log2 units");
         p.q = static_cast<const _Float16*>(q);
         p.out = static_cast<_Float16*>(out);
         p.k = k_pool; p.v = v_pool; p.scales = kv_scales; p.table = table_all;

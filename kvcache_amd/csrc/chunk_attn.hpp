@@ -79,11 +79,17 @@ __device__ __forceinline__ bool chunk_unit(const ChunkParams& p, ChunkUnit& u, i
     u.hk = (int)(blockIdx.x % (unsigned)p.Hkv);
     u.rows = u.ntok * u.hn;
     return u.row0 >= 0 && u.ntok > 0 && u.row0 <= p.rows - u.ntok && u.h0 >= 0 && u.hn > 0 && u.h0 <= p.group - u.hn &&
-           u.j0 >= 0 && u.pos0 >= 0 && u.tab >= 0 && u.c >= 0 && u.c < u.nc &&
+           u.j0 >= 0 && u.j0 < u.j1 && u.pos0 >= 0 && u.j1 - u.pos0 <= u.ntok && u.tab >= 0 && u.c >= 0 && u.c < u.nc &&
            (u.nc == 1 || (u.rec0 >= 0 && (long long)u.rec0 + (long long)u.nc * u.rows <= p.n_records)) &&
            (u.kind != kKindTile || p.n_wide == 0 ||
             (u.wide >= 0 && u.wkey >= 0 && u.wkey <= u.j0 && u.w0 >= u.wkey &&
              (long long)u.wide + (max(u.j1, u.w1) - u.wkey) <= p.n_wide));
+}
+
+// Block id of the unit's sequence at table position b, bounded by the table (no sum wraps below it).
+__device__ __forceinline__ int block_id(const ChunkParams& p, const ChunkUnit& u, int b) {
+    const unsigned at = (unsigned)u.tab + (unsigned)b, last = (unsigned)p.table_len - 1u;
+    return p.table[at < last ? at : last];
 }
 
 // Element offset of row r of the unit in q and out.
@@ -123,7 +129,7 @@ __global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkParams p) {
             const int n = min(kWave, hi - k0);
             const int key = k0 + min(lane, n - 1);
             const int b = key / p.block;
-            const int id = p.table[min(u.tab + b, p.table_len - 1)];
+            const int id = block_id(p, u, b);
             const size_t row = ((size_t)id * p.Hkv + u.hk) * p.block + (key - b * p.block);
             const char* kr = static_cast<const char*>(p.k) + row * (D * CB);
             float s = 0.f;
@@ -244,7 +250,7 @@ __device__ __forceinline__ f32x4 add_seen_nonfinite(const ChunkParams& p, const 
     const int bsh = __builtin_ctz((unsigned)p.block);
     const int first = max(u.j0, p.window > 0 ? pos - p.window + 1 : 0), last = min(u.j1 - 1, pos);
     for (int j = first; j <= last; ++j) {
-        const int id = p.table[min(u.tab + (j >> bsh), p.table_len - 1)];
+        const int id = block_id(p, u, j >> bsh);
         const size_t row = (((size_t)(unsigned)(id * p.Hkv + u.hk)) << bsh) + (j & (p.block - 1));
         const f16x4 v = *reinterpret_cast<const f16x4*>(static_cast<const _Float16*>(p.v) + row * D + d0);
         const u16x4 bits = __builtin_bit_cast(u16x4, v);
@@ -333,7 +339,7 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
     int ids = 0;
     auto load_ids = [&](int s) {
         const int t = min(first_tok(s + lane), j1 - 1);
-        ids = p.table[min(u.tab + (t >> bsh), p.table_len - 1)];
+        ids = block_id(p, u, t >> bsh);
     };
     struct Tile {
         u32x4 k[SUB][VL], v[SUB][VL];
@@ -425,7 +431,7 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
         if constexpr (Q8) {
             float ks = T.sc[0], vs = T.sc[1];
             if (!FULL && t0 + lane >= j1) ks = vs = 0.f;
-            float top = max_xor32(max_xor16(fmaxf(vs, 0.f)));
+            float top = max_xor32(max_xor16(fmaxf(fabsf(vs), 0.f)));  // (NaN: no part in it)
             top = fmaxf(top, dpp<0xB1>(top));
             top = fmaxf(top, dpp<0x4E>(top));
             top = fmaxf(top, dpp<0x141>(top));

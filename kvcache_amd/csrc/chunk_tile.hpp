@@ -83,7 +83,7 @@ __global__ __launch_bounds__(256) void widen_kernel(ChunkParams p) {
     const float kf = p.cap_log2 > 0.f ? p.cap_in : p.scale_log2;
     for (int k = k0 + threadIdx.x / LPR; k < k1; k += RPB) {
         const int b = k / p.block;
-        const int id = p.table[min(u.tab + b, p.table_len - 1)];
+        const int id = block_id(p, u, b);
         const size_t row = ((size_t)(unsigned)(id * p.Hkv + u.hk)) * p.block + (k - b * p.block);
         const size_t to = (size_t)u.hk * p.n_wide + u.wide + (k - u.wkey);
         const f32x2 s = *reinterpret_cast<const f32x2*>(p.scales + row * 2);
@@ -161,7 +161,7 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     auto first_tok = [&](int i) { return j0 + set_at(i) * kSetKeys + SR * wave; };
     int ids = 0;
     auto load_ids = [&](int i) {
-        if constexpr (!WIDE) ids = p.table[min(u.tab + (min(first_tok(i + lane), j1 - 1) >> bsh), p.table_len - 1)];
+        if constexpr (!WIDE) ids = block_id(p, u, min(first_tok(i + lane), j1 - 1) >> bsh);
     };
     auto row_of = [&](int t, int id) -> size_t {
         if constexpr (WIDE) return (size_t)u.hk * p.n_wide + u.wide + (t - u.wkey);

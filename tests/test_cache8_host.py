@@ -73,7 +73,7 @@ def attn(**kw):
 
 @pytest.mark.parametrize("kw", [dict(Hq=9), dict(Hkv=0), dict(BLOCK=0), dict(window=-1), dict(kv_dtype=5), dict(rows=-1),
                                 dict(n_units=-1), dict(n_tiles=-1), dict(ws_rows=(-1, 0)), dict(ws_rows=(0, -1)), dict(n_tiles=1), dict(scale=np.nan),
-                                dict(softcap=-1.0), dict(softcap=np.inf), dict(q=None), dict(out=P + 2),
+                                dict(softcap=-1.0), dict(softcap=np.inf), dict(scale=3e38), dict(softcap=1e-38, scale=100.0), dict(q=None), dict(out=P + 2),
                                 dict(k_pool=None), dict(v_pool=P + 8), dict(kv_scales=None), dict(kv_scales=P + 4),
                                 dict(table_all=None), dict(table_len=0), dict(work_dev=None),
                                 dict(ws_rows=(9, 0), workspace=(P + 4, 1 << 20))])
@@ -107,6 +107,7 @@ def test_plan_refuses():
     refused(N.KVC_ERR_ARG, ops.chunk_plan, [1], [1], 8, 2, 64, 16, tab_off=[0])
     refused(N.KVC_ERR_UNSUPPORTED, ops.chunk_plan, [1], [1], 8, 2, 72, 16)
     refused(N.KVC_ERR_UNSUPPORTED, ops.chunk_plan, [0, 0], [2 ** 31 - 1] * 2, 8, 2, 64, 1)
+    refused(N.KVC_ERR_UNSUPPORTED, ops.chunk_plan, [1], [17], 8, 2, 64, 16, tab_off=[2 ** 31 - 2, 2 ** 31 - 1])
     L = N.lib()
     import ctypes as C
     n = [C.c_int(0) for _ in range(4)]

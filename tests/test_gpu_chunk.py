@@ -286,6 +286,58 @@ def test_captured_launch_replays_other_plans(D, kv):
     check(L.kvc_graph_destroy(ex))
 
 
+@pytest.mark.parametrize("kv", ALL, ids=NAME.get)
+def test_two_captured_launches_share_a_workspace(kv):
+    """Replayed in turn on one stream, with other contents in the workspace now and then."""
+    bs = [Batch([1, 70, 2], [4000, 2500, 900], 8, 2, 64, 16, kv, seed=70), Batch([3, 1, 33], [900, 6000, 1500], 8, 2, 64, 16, kv, seed=71)]
+    want = [b.run() for b in bs]
+    assert all(b.plan[3][0] > 0 for b in bs)
+    n = max(ops.chunk_workspace_size(8, 2, 64, b.plan[3]) for b in bs)
+    ws, st, L = DeviceBuffer(n), Stream(), lib()
+    graphs = []
+    for b in bs:
+        q, k, v, sc, tab, w = b.bufs
+        out, ex = dev(np.zeros((b.rows, 8, 64), np.float16)), C.c_void_p()
+        check(L.kvc_graph_begin(st.handle))
+        ops.paged_chunk_attn(q, out, k, v, None if kv == KVC_F16 else sc, tab, len(b.table), w, *b.plan[1:], b.rows, 8, 2,
+                             64, 16, 0.125, kv_dtype=kv, workspace=ws, stream=st.handle)
+        check(L.kvc_graph_end(st.handle, C.byref(ex)))
+        graphs.append((ex, out))
+    rng = np.random.default_rng(0)
+    for i in (0, 1, 1, 0, 0, 1):
+        if i == 0:
+            ws.upload(rng.integers(0, 256, n, dtype=np.uint8))
+        ex, out = graphs[i]
+        out.upload(np.zeros((bs[i].rows, 8, 64), np.float16))
+        check(L.kvc_graph_launch(ex, st.handle))
+        st.synchronize()
+        assert (host(out, np.float16, want[i].shape) == want[i]).all()
+    for ex, _ in graphs:
+        check(L.kvc_graph_destroy(ex))
+
+
+@pytest.mark.parametrize("kv", ALL, ids=NAME.get)
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_output_in_place_of_the_queries(D, kv):
+    b = Batch([1, 70, 2], [3000, 90, 900], 8, 2, D, 16, kv, seed=72)
+    want = b.run()
+    q, k, v, sc, tab, w = b.bufs
+    ops.paged_chunk_attn(q, q, k, v, None if kv == KVC_F16 else sc, tab, len(b.table), w, *b.plan[1:], b.rows, 8, 2, D, 16,
+                         D ** -0.5, kv_dtype=kv)
+    synchronize()
+    assert (host(q, np.float16, want.shape) == want).all()
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_signed_scales(D):
+    """Codes and scale of opposite sign stand for the same row."""
+    b = Batch([1, 70], [700, 90], 8, 2, D, 16, KVC_I8, seed=73)
+    for i in (0, 1):
+        b.pools[i] = np.where(b.pools[i] == -128, b.pools[i], -b.pools[i]).astype(np.int8)
+    b.scales = -b.scales
+    b.check()
+
+
 @pytest.mark.parametrize("kv", [KVC_I8, KVC_E4M3], ids=NAME.get)
 def test_cache_past_32_bits(kv):
     """Pools of more than 2^32 bytes: blocks at their far end are found."""
