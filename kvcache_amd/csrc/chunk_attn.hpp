@@ -202,19 +202,27 @@ __global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkParams p) {
 //     codes at a time and turned into fp16 exactly; lane l's 16 codes are dims 64 j + 16 (l /
 //     16) .. + 15, two k steps of the product, and q lies in that order of dims.  The key's
 //     scale multiplies the score.
-//   softmax online in log2 units, fp32.
+//   softmax online in log2 units, fp32: p = 2^(s - reference).  The reference lags: it moves to the
+//     row's maximum when a score passes it by more than kRowLag, so most tiles need no maximum
+//     over the row's lanes and no rescaled O (48 sequences of 1 to 300 tokens, 14q/2kv, D 64: 16.1
+//     -> 15.7 us).
 //   O[row][dim] += P V: P is the lane's own scores' probabilities (keys 4 g + r of two
 //     subtiles, g = l / 16), V is read back transposed: 8-bit rows with ds_read_b64_tr_b8 (of
 //     16 lanes, lane i receives byte i % 8 of the 8 bytes that lanes 2 j + i / 8 address, j =
 //     0 .. 7: one dim of eight keys), fp16 rows with ds_read_b64_tr_b16.  The key's V scale
-//     goes onto its probability, in fp32 and before the rounding to fp16, in units of 2^(E - 15)
-//     with 2^E above every V scale met so far (O is kept in them): products of up to 2^15, so
-//     that fp16 has all its bits down to 2^-29 of the largest (in units of 2^E, V rows of sizes
-//     2^+-9 cost 2^-8 where a row's weight lay on small ones).  fp16 caches: probabilities are
-//     kept times 2^15 for the same reason.
+//     goes onto its probability, in fp32 and before the rounding to fp16, in units of 2^(E - 11)
+//     with 2^E above every V scale met so far (O is kept in them): at the reference 2^11, at most
+//     2^15, so that fp16 has all its bits down to 2^-25 of the largest (in units of 2^E, V rows of
+//     sizes 2^+-9 cost 2^-8 where a row's weight lay on small ones).  fp16 caches: probabilities
+//     are kept times 2^11 for the same reason.  8-bit caches: what the rounding to fp16 loses of a
+//     probability follows as a second product, so that the output is as exact as its own rounding
+//     (2.1e-4 of 64 bits instead of 3.0e-4; 1 to 6% of the time: the mixed batch 15.7 -> 16.6 us).
+//     An Inf in an fp16 cache would become NaN by it.
+// D 64 takes three waves a SIMD (168 registers): at four it spilled 76 bytes, and 128 single tokens
+// of MHA took 20.6 us instead of 17.3, the mixed batch 18.5 instead of 16.1.
 // LDS rows are 16-byte pieces permuted by the row, so that the sixteen rows one operand read
 // touches at the same piece lie on different banks.
-constexpr int kProbBits = 15;  // probabilities (times V scales) go up to 2^15
+constexpr int kProbBits = 11, kRowLag = 4;  // probabilities (times V scales) at the reference, and how far they pass it
 
 constexpr int kStreamWaves = 4;  // waves of a workgroup
 
@@ -400,18 +408,18 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
     }
     const bool cap = p.cap_log2 > 0.f;
     const float to_log2 = cap ? p.cap_in : p.scale_log2;
-    float m[R], l[R];
+    float ref[R], lim[R], l[R];  // lim: a score further above ref moves it (none met yet: any)
     f32x4 O[R][NT];
     int E = -126;
 #pragma unroll
     for (int a = 0; a < R; ++a) {
-        m[a] = -FLT_MAX;
+        ref[a] = 0.f;
+        lim[a] = -FLT_MAX;
         l[a] = 0.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) O[a][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    auto fence = [] { asm volatile("" ::: "memory"); };
     bool bad = false;  // this wave cleared elements of V in tiles that some row does not see whole
     // FULL: every key of the tile is seen by every row
     auto consume = [&](int k, auto full_tag) {
@@ -427,7 +435,7 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
                 for (int h = 0; h < SUB; ++h) clear_nonfinite(T.v[h]);
             }
         }
-        float efac = 1.f;
+        int En = E;
         if constexpr (Q8) {
             float ks = T.sc[0], vs = T.sc[1];
             if (!FULL && t0 + lane >= j1) ks = vs = 0.f;
@@ -437,9 +445,7 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
             top = fmaxf(top, dpp<0x141>(top));
             top = fmaxf(top, dpp<0x140>(top));
             const int e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) : -126;
-            const int En = uniform(max(E, e));
-            efac = __builtin_amdgcn_ldexpf(1.f, E - En);
-            E = En;
+            En = uniform(max(E, e));
             s_k[lane] = ks * to_log2;
             s_v[lane] = __builtin_amdgcn_ldexpf(vs, kProbBits - En);
         }
@@ -466,7 +472,6 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
         for (int h = 0; h < SUB; ++h) {
             const int r = 16 * h + n16;
             f16x8v ka[KD];
-            fence();
             if constexpr (Q8) {
 #pragma unroll
                 for (int j = 0; j < KD / 2; ++j) {
@@ -487,65 +492,73 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
                 S[a][h] = acc;
             }
         }
-        // (the fences keep operand reads of later steps from being held in registers through earlier
-        // ones: without them D 64 took 174 registers, two waves a SIMD instead of four)
-        fence();
-#pragma unroll
-        for (int h = 0; h < SUB; ++h) {
-            f32x4 kf;
-            if constexpr (Q8) kf = *reinterpret_cast<const f32x4*>(s_k + 16 * h + 4 * g4);
-#pragma unroll
-            for (int a = 0; a < R; ++a)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) S[a][h][r] *= Q8 ? kf[r] : to_log2;
-        }
-        f16x8v pa[R][SUB / 2];
-        float cr[R][4];
+        f16x8v pa[R][SUB / 2], pl[R][SUB / 2];
 #pragma unroll
         for (int a = 0; a < R; ++a) {
-            if (cap) {
-#pragma unroll
-                for (int i = 0; i < 4 * SUB; ++i)
-                    S[a][i >> 2][i & 3] = capped(S[a][i >> 2][i & 3], 1.f, p.cap_log2);
-            }
-            // key t0 + 16 h + 4 g + r is seen when low < 16 h + r <= lim
-            const int lim = min(pos[a], j1 - 1) - t0 - 4 * g4;
+            // key t0 + 16 h + 4 g + r is seen when low < 16 h + r <= last
+            const int last = min(pos[a], j1 - 1) - t0 - 4 * g4;
             const int low = (p.window > 0 ? pos[a] - p.window : -1) - t0 - 4 * g4;
             auto seen = [&](int i) {
                 const int c = 16 * (i >> 2) + (i & 3);
-                return FULL || (c <= lim && c > low);
+                return FULL || (c <= last && c > low);
             };
+            // scores above the reference, in log2 units
+            auto each = [&](auto&& f) {
+#pragma unroll
+                for (int h = 0; h < SUB; ++h) {
+                    f32x4 kf;
+                    if constexpr (Q8) kf = *reinterpret_cast<const f32x4*>(s_k + 16 * h + 4 * g4);
+                    else kf[0] = kf[1] = kf[2] = kf[3] = to_log2;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[a][h][r] = f(S[a][h][r], kf[r]);
+                }
+            };
+            if (cap) each([&](float x, float f) { return capped(x, f, p.cap_log2) - ref[a]; });
+            else each([&](float x, float f) { return __builtin_fmaf(x, f, -ref[a]); });
             float mx = -FLT_MAX;
 #pragma unroll
-            for (int i = 0; i < 4 * SUB; ++i) mx = seen(i) ? fmaxf(mx, S[a][i >> 2][i & 3]) : mx;
-            mx = max_xor32(max_xor16(mx));
-            const float mn = fmaxf(m[a], mx), corr = fast_exp2(m[a] - mn);
-            // (a little further for scores whose last bit is more than 1: p has to stay below 2^16)
-            const float ref = Q8 ? mn : mn - (float)kProbBits + fabsf(mn) * 0x1p-23f;
-            float ps = 0.f;
-            fence();
+            for (int i = 0; i < 4 * SUB; ++i) {
+                const float x = seen(i) ? S[a][i >> 2][i & 3] : -__builtin_inff();
+                S[a][i >> 2][i & 3] = x;
+                mx = fmaxf(mx, x);
+            }
+            if (__builtin_expect(__any(mx > lim[a]) || En != E, 0)) {
+                mx = max_xor32(max_xor16(mx));
+                const bool move = mx > lim[a];
+                // (a little further for scores whose last bit is more than 1: p has to stay within fp16)
+                const float by = move ? mx + fabsf(ref[a] + mx) * 0x1p-22f : 0.f;
+                const float corr = lim[a] > -FLT_MAX ? fast_exp2(-by) : 1.f;
+                ref[a] += by;
+                lim[a] = move ? (float)kRowLag : lim[a];
+                l[a] *= corr;
+#pragma unroll
+                for (int i = 0; i < 4 * SUB; ++i) S[a][i >> 2][i & 3] -= by;
+                const float oc = Q8 ? __builtin_amdgcn_ldexpf(corr, E - En) : corr;
+                // row 4 g + r of the output belongs to the lane that holds row 4 g + r of the scores
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float cr = __int_as_float(__builtin_amdgcn_ds_bpermute((4 * g4 + r) << 2, __float_as_int(oc)));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) O[a][nt][r] *= cr;
+                }
+            }
 #pragma unroll
             for (int h = 0; h < SUB; ++h) {
                 f32x4 vf;
                 if constexpr (Q8) vf = *reinterpret_cast<const f32x4*>(s_v + 16 * h + 4 * g4);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float e = seen(4 * h + r) ? fast_exp2(S[a][h][r] - ref) : 0.f;
-                    ps += e;
-                    pa[a][h >> 1][4 * (h & 1) + r] = (_Float16)(!Q8 ? e : seen(4 * h + r) ? e * vf[r] : 0.f);
+                    const float e = fast_exp2(Q8 ? S[a][h][r] : S[a][h][r] + (float)kProbBits);
+                    l[a] += e;
+                    const float x = !Q8 ? e : seen(4 * h + r) ? e * vf[r] : 0.f;
+                    pa[a][h >> 1][4 * (h & 1) + r] = (_Float16)x;
+                    if constexpr (Q8) pl[a][h >> 1][4 * (h & 1) + r] = (_Float16)(x - (float)(_Float16)x);
                 }
             }
-            l[a] = __builtin_fmaf(l[a], corr, ps);
-            m[a] = mn;
-            const float oc = Q8 ? corr * efac : corr;
-            // row 4 g + r of the output belongs to the lane that holds row 4 g + r of the scores
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                cr[a][r] = __int_as_float(__builtin_amdgcn_ds_bpermute((4 * g4 + r) << 2, __float_as_int(oc)));
         }
+        E = En;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            if ((nt & 1) == 0) fence();
             f16x8v vv[SUB / 2];
 #pragma unroll
             for (int s = 0; s < SUB / 2; ++s) {
@@ -561,11 +574,11 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
             }
 #pragma unroll
             for (int a = 0; a < R; ++a) {
-                f32x4 pv = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < SUB / 2; ++s) pv = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa[a][s], vv[s], pv, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) O[a][nt][r] = __builtin_fmaf(O[a][nt][r], cr[a][r], pv[r]);
+                for (int s = 0; s < SUB / 2; ++s) {
+                    O[a][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa[a][s], vv[s], O[a][nt], 0, 0, 0);
+                    if constexpr (Q8) O[a][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[a][s], vv[s], O[a][nt], 0, 0, 0);
+                }
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -601,7 +614,7 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
         for (int a = 0; a < R; ++a) {
             const float lt = sum_xor32(sum_xor16(l[a]));
             if (lane < 16) {
-                s_ml[wave][16 * a + lane][0] = m[a];
+                s_ml[wave][16 * a + lane][0] = lim[a] > -FLT_MAX ? ref[a] : -FLT_MAX;
                 s_ml[wave][16 * a + lane][1] = lt;
                 s_ml[wave][16 * a + lane][2] = Q8 ? __builtin_amdgcn_ldexpf(1.f, E - kProbBits) : 1.f;
             }
@@ -695,7 +708,7 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
 }
 
 template <int D, int CT>
-__global__ __launch_bounds__(kStreamWaves * kWave, D == 64 ? 4 : 2) void chunk_stream_kernel(ChunkParams p) {
+__global__ __launch_bounds__(kStreamWaves * kWave, D == 64 ? 3 : 2) void chunk_stream_kernel(ChunkParams p) {
     __shared__ __attribute__((aligned(16))) char lds[StreamShape<D, CT>::kBytes];
     ChunkUnit u;
     if (!chunk_unit(p, u, max(p.work[kHdrTiles], 0)) || u.kind != kKindRows) return;
