@@ -44,26 +44,28 @@ __device__ __forceinline__ f16x8 codes_to_f16x8(u32x2 x) {
 }
 
 // Scale of a row from the bits of max|x| (as an integer, whose order is that of the
-// magnitudes with NaN above Inf), and the factor that turns values into codes.
+// magnitudes with NaN above Inf), and the factor that turns values into codes, as a sum of
+// two floats: with one alone the quotient would be rounded twice.
 template <int CT>
-__device__ __forceinline__ void row_scale(unsigned amax_bits, float& s, float& inv) {
+__device__ __forceinline__ void row_scale(unsigned amax_bits, float& s, f32x2& inv) {
     constexpr float kTop = CT == kCacheI8 ? 127.f : 448.f;
     const float a = __uint_as_float(amax_bits);
     s = a / kTop;
-    inv = kTop / a;
-    if (amax_bits < 0x0D800000u) s = inv = 0.f;  // 2^-100
+    inv[0] = kTop / a;
+    inv[1] = __builtin_fmaf(-inv[0], a, kTop) * inv[0] * (1.f / kTop);
+    if (amax_bits < 0x0D800000u) s = inv[0] = inv[1] = 0.f;  // 2^-100
     if (amax_bits >= 0x7F800000u) {
         s = __builtin_nanf("");
-        inv = 0.f;
+        inv[0] = inv[1] = 0.f;
     }
 }
 
 // Eight values times inv as codes.  (inv 0 with an Inf or NaN among x: codes 0.)
 template <int CT>
-__device__ __forceinline__ u32x2 values_to_codes(const float (&x)[8], float inv) {
+__device__ __forceinline__ u32x2 values_to_codes(const float (&x)[8], f32x2 inv) {
     float y[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = inv == 0.f ? 0.f : x[e] * inv;
+    for (int e = 0; e < 8; ++e) y[e] = inv[0] == 0.f ? 0.f : __builtin_fmaf(x[e], inv[0], x[e] * inv[1]);
     u32x2 c;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {

@@ -119,10 +119,10 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
     auto first_key = [&](int pos) { return window > 0 ? std::max(0, pos - window + 1) / 64 * 64 : 0; };
     // Tiles reach about three times the rate of units of 16 rows, but take a launch or two more (merge;
     // 8-bit caches: widening).  One sequence, int8 (fp16), units of 16 and tiles: 14q/2kv, D 64, 400
-    // tokens behind 1000 (1.7 GFLOP) 17 and 25 us (15 and 20), 1000 behind 1000 (5.4) 28 and 30 (25 and
-    // 24), 400 behind 4000 (6.0) 41 and 31 (36 and 24); 32q/8kv, D 128, 64 behind 4000 (4.2) 23 and 33
-    // (23 and 25), 500 behind 500 (6.1) 30 and 33 (28 and 27), 400 behind 1000 (7.9) 38 and 36 (36 and
-    // 28), 150 behind 4000 (10) 50 and 40 (49 and 31).
+    // tokens behind 1000 (1.7 GFLOP) 16 and 25 us (12 and 20), 1000 behind 1000 (5.4) 30 and 30 (28 and
+    // 24), 400 behind 4000 (6.0) 40 and 31 (29 and 24); 32q/8kv, D 128, 64 behind 4000 (4.2) 24 and 33
+    // (23 and 25), 500 behind 500 (6.1) 31 and 34 (27 and 27), 400 behind 1000 (7.9) 38 and 36 (35 and
+    // 29), 150 behind 4000 (10) 51 and 41 (49 and 32).
     bool tiled = false;
     if (matrix_path(D, BLOCK)) {
         double flops = 0;
