@@ -406,11 +406,20 @@ __device__ __forceinline__ void stream_unit(const ChunkParams& p, const ChunkUni
         for (int d = 0; d < KD; ++d)
             qb[a][d] = *reinterpret_cast<const f16x8v*>(q + (Q8 ? 64 * (d >> 1) + 16 * g4 + 8 * (d & 1) : 32 * d + 8 * g4));
     }
+    // q has to be there before the loop: counted as under way in it, its loads made every tile wait for
+    // the next one's rows before its first product (4 sequences of 8000 to 32768, 14q/2kv: 16.4 us,
+    // 15.2 so; at D 128, where HBM is the bound, 200 sequences 73.4 and 74.3)
+    if constexpr (D == 64) {
+#pragma unroll
+        for (int a = 0; a < R; ++a)
+#pragma unroll
+            for (int d = 0; d < KD; ++d) asm volatile("" : "+v"(qb[a][d]));
+    }
     const bool cap = p.cap_log2 > 0.f;
     const float to_log2 = cap ? p.cap_in : p.scale_log2;
     float ref[R], lim[R], l[R];  // lim: a score further above ref moves it (none met yet: any)
     f32x4 O[R][NT];
-    int E = -126;
+    int E = -126;                  // V scales met so far are below 2^E
 #pragma unroll
     for (int a = 0; a < R; ++a) {
         ref[a] = 0.f;
