@@ -44,16 +44,16 @@ struct PlanUnit {
     long long cost;
 };
 
-// Keys per chunk of the units of 16 rows, `keys` of them over all units and KV heads.  Two
-// workgroups fit a CU (512), and chunks of 512 keys keep them in flight; below that a batch is
-// still cut for one workgroup a CU down to 256 keys (one round of four waves).  int8, 32q/8kv, D
-// 128: one sequence of 4000 38.4 us whole, 15.2 in chunks of 1024, 10.4 in 256; 64 of 32..4096 43.4
-// whole, 34.6 for 256 workgroups, 30.8 for 512; 16 of 4000 (8q/8kv, D 64) 33 whole, 24.1 and 22.9.
+// Keys per chunk of the units of 16 rows, `keys` of them over all units and KV heads.  A batch is cut
+// for one workgroup a CU (256) down to 256 keys (one round of four waves), for two down to 1024.
+// int8, 32q/8kv, D 128: one sequence of 4000 38.4 us whole, 15.2 in chunks of 1024, 10.7 in 256; 64 of
+// 32..4096 33.7 for 256 workgroups, 27.9 in chunks of 1024, 30.6 of 512; 128 of 16..2048 (8q/8kv, D 64,
+// e4m3) 16.4, 15.1 and 16.8; 48 of 32..4096, 1 to 300 tokens (14q/2kv, D 64) 21.8, 17.1 and 16.9.
 // At most 32 chunks of a sequence, whose arrivals are served one after the other (one of 20000,
-// 8q/8kv: 13.3 us in 32 chunks, 17.8 in 40, 19.8 in 63).
+// 8q/8kv: 12.3 us in 32 chunks, 13.4 in 24, 17.8 in 40).
 long long stream_chunk(long long keys, int longest) {
     const long long one = (keys + 255) / 256, two = (keys + 511) / 512;
-    const long long c = std::max(256LL, std::min(one, std::max(two, 512LL)));
+    const long long c = std::max(256LL, std::min(one, std::max(two, 1024LL)));
     return (std::max<long long>(c, (longest + 31) / 32) + 63) / 64 * 64;
 }
 
