@@ -135,6 +135,7 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
         tiled = knob >= 0 ? knob == 1 : flops >= (D == 64 ? 5.6e9 : 7e9) * (kv_dtype == KVC_F16 ? 0.6 : 1.0);
     }
     std::vector<Tile> tiles;
+    tiles.reserve(N);
     long long row = 0, tab = 0, stream_keys = 0;
     int stream_longest = 0;
     wide = 0;
@@ -164,6 +165,7 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
     }
     records = 0;
     const long long chunk[2] = {stream_chunk(stream_keys * Hkv, stream_longest), tile_chunk(tiles, Hkv, D)};
+    units.reserve(tiles.size() + tiles.size() / 4);
     for (const Tile& t : tiles) {
         const int len = t.j1 - t.j0;
         int nc = chunks_of(len, chunk[t.kind == kKindTile]);
@@ -205,9 +207,18 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
             }
             a = std::max(b, a + 1);
         }
-    std::stable_sort(units.begin(), units.end(), [](const PlanUnit& a, const PlanUnit& b) {
-        return a.f[kFKind] != b.f[kFKind] ? a.f[kFKind] > b.f[kFKind] : a.cost > b.cost;
-    });
+}
+
+// The list's order: tiles first, then by what a unit computes, the longest first (so that the last
+// workgroups to start are short).
+std::vector<int> unit_order(const std::vector<PlanUnit>& units) {
+    std::vector<std::pair<long long, int>> key(units.size());
+    for (size_t i = 0; i < units.size(); ++i)
+        key[i] = {-(units[i].cost + (units[i].f[kFKind] == kKindTile ? 1LL << 61 : 0)), (int)i};
+    std::sort(key.begin(), key.end());
+    std::vector<int> order(units.size());
+    for (size_t i = 0; i < units.size(); ++i) order[i] = key[i].second;
+    return order;
 }
 
 template <typename F>
@@ -306,7 +317,10 @@ int kvc_chunk_plan(const int* host_q_lens, const int* host_kv_lens, const int* h
         work[kHdrUnits] = *n_units;
         work[kHdrTiles] = *n_tiles;
         work[kHdrRecords] = *n_records;
-        for (size_t i = 0; i < units.size(); ++i) std::copy(units[i].f, units[i].f + kChunkInts, work + (i + 1) * kChunkInts);
+        for (const int i : unit_order(units)) {
+            work += kChunkInts;
+            std::copy(units[i].f, units[i].f + kChunkInts, work);
+        }
         return KVC_OK;
     });
 }

@@ -10,7 +10,7 @@ drivers call the CUDA launchers.
 """
 from __future__ import annotations
 
-from ._native import KVC_E4M3, KVC_ERR_ARG, KVC_F16, KVC_F32, KVC_I8, KvcError, check, lib
+from ._native import KVC_E4M3, KVC_ERR_ARG, KVC_F16, KVC_F32, KVC_I8, KVC_OK, KvcError, check, lib
 from .device import DeviceBuffer
 
 __all__ = [
@@ -231,13 +231,17 @@ def chunk_plan(q_lens, kv_lens, Hq, Hkv, D, BLOCK, *, tab_off=None, kv_dtype=KVC
     nu, nt, nr, nw = (C.c_int(0) for _ in range(4))
     L = lib()
 
-    def plan(work, cap):
-        check(L.kvc_chunk_plan(q.ctypes.data, t.ctypes.data, tp, len(q), Hq, Hkv, D, BLOCK, kv_dtype, window, work, cap,
-                               C.byref(nu), C.byref(nt), C.byref(nr), C.byref(nw)))
+    def plan(work):
+        return L.kvc_chunk_plan(q.ctypes.data, t.ctypes.data, tp, len(q), Hq, Hkv, D, BLOCK, kv_dtype, window,
+                                work.ctypes.data, len(work), C.byref(nu), C.byref(nt), C.byref(nr), C.byref(nw))
 
-    plan(None, 0)
-    work = np.zeros((nu.value, 16), dtype=np.int32)
-    plan(work.ctypes.data, nu.value)
+    work = np.empty((64 + 4 * len(q), 16), dtype=np.int32)
+    rc = plan(work)
+    if rc != KVC_OK and nu.value > len(work):
+        work = np.empty((nu.value, 16), dtype=np.int32)
+        rc = plan(work)
+    check(rc)
+    work = work[:nu.value]
     return work, nu.value, nt.value, (nr.value, nw.value)
 
 
