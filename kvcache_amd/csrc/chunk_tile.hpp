@@ -258,10 +258,13 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     // it.  S[i] is key t0 + 8 (i / 4) + 4 h + i % 4; the subtile's factors begin at kf.
     auto settle = [&](f32x16& S, const float* kf, int t0, auto masked_tag) {
         if constexpr (WIDE) scale_scores(S, kf[fl]);
+        // (capped: S becomes w = 1 / (1 + e^(2x / cap)), the score is cap - 2 cap w)
         if constexpr (CAP) {
+            const float f = WIDE ? 1.f : p.cap_in;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) S[i] = capped(S[i], WIDE ? 1.f : p.cap_in, p.cap_log2);
+            for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_rcpf(1.f + fast_exp2(S[i] * f));
         }
+        constexpr float kNone = CAP ? __builtin_inff() : -__builtin_inff();
         if constexpr (decltype(masked_tag)::value) {
             // seen when low < 8 (i / 4) + i % 4 <= lim
             const int lim = min(pos, j1 - 1) - t0 - 4 * h;
@@ -269,12 +272,13 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int c = 8 * (i >> 2) + (i & 3);
-                S[i] = c <= lim && c > low ? S[i] : -__builtin_inff();
+                S[i] = c <= lim && c > low ? S[i] : kNone;
             }
         }
-        float mx = -FLT_MAX;
+        float mx = CAP ? FLT_MAX : -FLT_MAX;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[i]);
+        for (int i = 0; i < 16; ++i) mx = CAP ? fminf(mx, S[i]) : fmaxf(mx, S[i]);
+        if constexpr (CAP) mx = __builtin_fmaf(mx, -2.f * p.cap_log2, p.cap_log2);
         // (rare: said so, since the compiler otherwise copies O for its sake on every tile)
         if (__builtin_expect(__any(mx * sl2 > thr), 0)) {
             mx = max_xor32(mx) * sl2;
@@ -294,10 +298,11 @@ __device__ __forceinline__ void tile_unit(const ChunkParams& p, const ChunkUnit&
     // probabilities and P V of a subtile, the n-th of its set
     auto weigh = [&](const f32x16& S, const char* vd, int n) {
         f16x8v pb[2];
+        const float off = CAP ? p.cap_log2 - ref : -ref;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) pb[t][j] = (_Float16)fast_exp2(__builtin_fmaf(S[8 * t + j], sl2, -ref));
+            for (int j = 0; j < 8; ++j) pb[t][j] = (_Float16)fast_exp2(__builtin_fmaf(S[8 * t + j], CAP ? -2.f * p.cap_log2 : sl2, off));
             const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
             l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 0, 1), one, l, false);
             l = __builtin_amdgcn_fdot2(__builtin_shufflevector(pb[t], pb[t], 2, 3), one, l, false);
