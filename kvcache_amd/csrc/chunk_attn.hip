@@ -44,6 +44,9 @@ struct PlanUnit {
     long long cost;
 };
 
+// Chunks of `len` keys at a target of c (up to 1.5 c stay whole).
+int chunks_of(long long len, long long c) { return len > c * 3 / 2 ? (int)((len + c - 1) / c) : 1; }
+
 // Keys per chunk of the units of 16 rows, `keys` of them over all units and KV heads.  A batch is cut
 // for one workgroup a CU (256) down to 256 keys (one round of four waves), for two down to 1024.
 // int8, 32q/8kv, D 128: one sequence of 4000 38.4 us whole, 15.2 in chunks of 1024, 10.7 in 256; 64 of
@@ -51,14 +54,32 @@ struct PlanUnit {
 // e4m3) 16.4, 15.1 and 16.8; 48 of 32..4096, 1 to 300 tokens (14q/2kv, D 64) 21.8, 17.1 and 16.9.
 // At most 32 chunks of a sequence, whose arrivals are served one after the other (one of 20000,
 // 8q/8kv: 12.3 us in 32 chunks, 13.4 in 24, 17.8 in 40).
-long long stream_chunk(long long keys, int longest) {
+// A few workgroups more than the card holds at once (D 128: 512) are a round of their own where all are
+// about as long: then longer chunks that fit are taken (24 of 4000, 32q/8kv, D 128, int8: 57.0 -> 49.1
+// us, of 1000..8000 48.8 -> 39.5; at D 64, three workgroups a CU, it gained nothing).
+long long stream_chunk(const std::vector<Tile>& tiles, int Hkv, int D) {
+    long long keys = 0, longest = 0;
+    for (const Tile& t : tiles) {
+        if (t.kind == kKindTile) continue;
+        keys += t.j1 - t.j0;
+        longest = std::max<long long>(longest, t.j1 - t.j0);
+    }
+    keys *= Hkv;
     const long long one = (keys + 255) / 256, two = (keys + 511) / 512;
-    const long long c = std::max(256LL, std::min(one, std::max(two, 1024LL)));
-    return (std::max<long long>(c, (longest + 31) / 32) + 63) / 64 * 64;
+    long long c = std::max(256LL, std::min(one, std::max(two, 1024LL)));
+    c = (std::max<long long>(c, (longest + 31) / 32) + 63) / 64 * 64;
+    auto units = [&](long long size) {
+        long long u = 0;
+        for (const Tile& t : tiles)
+            if (t.kind != kKindTile) u += chunks_of(t.j1 - t.j0, size);
+        return u * Hkv;
+    };
+    const long long n = units(c);
+    if (D == 128 && c < longest && n > 512 && n <= 640 && 4 * keys >= 3 * n * c)
+        for (long long size = c + 64; size <= 2 * c; size += 64)
+            if (units(size) <= 512) return size;
+    return c;
 }
-
-// Chunks of `len` keys at a target of c (up to 1.5 c stay whole).
-int chunks_of(long long len, long long c) { return len > c * 3 / 2 ? (int)((len + c - 1) / c) : 1; }
 
 // Keys per chunk of the tiles (INT_MAX: whole): the shortest estimate among whole tiles and chunks
 // for one, two or three rounds of the card's workgroups.  A set of 64 keys takes a tile of 256 rows
@@ -136,8 +157,7 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
     }
     std::vector<Tile> tiles;
     tiles.reserve(N);
-    long long row = 0, tab = 0, stream_keys = 0;
-    int stream_longest = 0;
+    long long row = 0, tab = 0;
     wide = 0;
     for (int s = 0; s < N; ++s) {
         const int nq = q_lens[s], nk = kv_lens[s];
@@ -153,10 +173,6 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
                        std::min(hstep, group - h), 0, 0, (int)tab, (int)std::min<long long>(wide, INT_MAX), key0};
                 t.j1 = t.pos0 + t.ntok;
                 t.j0 = first_key(t.pos0);
-                if (!tile) {
-                    stream_keys += t.j1 - t.j0;
-                    stream_longest = std::max(stream_longest, t.j1 - t.j0);
-                }
                 tiles.push_back(t);
             }
         if (tile && kv_dtype != KVC_F16) wide += nk - key0;
@@ -164,7 +180,7 @@ void plan_units(const int* q_lens, const int* kv_lens, const int* tab_off, int N
         if (!tab_off) tab += ((long long)nk + BLOCK - 1) / BLOCK;
     }
     records = 0;
-    const long long chunk[2] = {stream_chunk(stream_keys * Hkv, stream_longest), tile_chunk(tiles, Hkv, D)};
+    const long long chunk[2] = {stream_chunk(tiles, Hkv, D), tile_chunk(tiles, Hkv, D)};
     units.reserve(tiles.size() + tiles.size() / 4);
     for (const Tile& t : tiles) {
         const int len = t.j1 - t.j0;
