@@ -412,8 +412,8 @@ int kvc_read_kv(void* k, void* v, const void* k_pool, const void* v_pool, const 
  * count as Inf.
  *
  * kvc_chunk_plan (host, once per step): cuts the batch into units and writes them into `work`
- *   (host memory of capacity * 16 ints; NULL: only counts).  capacity and *n_units are in
- *   entries of 16 ints, the list's header (entry 0) included; *n_tiles of the units are tiles of
+ *   (host memory of capacity * 16 ints; NULL: only counts; too small: KVC_ERR_ARG, the counts
+ *   set).  capacity and *n_units are in entries of 16 ints, the list's header (entry 0) included; *n_tiles of the units are tiles of
  *   many rows; *n_records is the partial rows of split key ranges, *n_wide the keys that tiles
  *   over an 8-bit cache hold as fp16 in the workspace.  host_tab_off (N + 1, NULL: tables packed
  *   in sequence order) locates each sequence's table in table_all.  The caller copies the list

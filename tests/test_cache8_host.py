@@ -181,6 +181,18 @@ def test_tile_knob():
         assert L.kvc_set_tuning(b"chunk_tiles", bad) == N.KVC_ERR_ARG
 
 
+def test_plan_larger_than_its_first_buffer():
+    """The binding's second call: many more units than four a sequence."""
+    work, nu, nt, (nr, nw) = ops.chunk_plan([3000], [3000], 14, 2, 64, 10)
+    assert nu > 68 and work.shape == (nu, 16) and work[0, 0] == nu and (work[1:, 2] > 0).all()
+    n = [C.c_int(0) for _ in range(4)]
+    q = np.array([3000], np.int32)
+    small = np.zeros((4, 16), np.int32)
+    assert N.lib().kvc_chunk_plan(q.ctypes.data, q.ctypes.data, None, 1, 14, 2, 64, 10, N.KVC_I8, 0, small.ctypes.data, 4,
+                                  *map(C.byref, n)) == N.KVC_ERR_ARG
+    assert n[0].value == nu and (small == 0).all()
+
+
 def test_plan_of_an_empty_batch():
     for q, t in (([], []), ([0, 0], [0, 30])):
         work, nu, nt, rows = ops.chunk_plan(q, t, 8, 2, 64, 16)
