@@ -402,8 +402,9 @@ int kvc_read_kv(void* k, void* v, const void* k_pool, const void* v_pool, const 
  * sequence s brings q_lens[s] >= 0 new tokens (1: a decode step), whose K and V are already in
  * the cache, and then holds kv_lens[s] >= q_lens[s] tokens.  Token i of it sits at position
  * p = kv_lens[s] - q_lens[s] + i and attends to keys max(0, p - window + 1) .. p (window 0: from
- * 0); scores are scale * q.k, with softcap > 0 softcap * tanh(score / softcap).  q and out are
- * [rows, Hq, D] fp16, the sequences' tokens one after the other; statistics are fp32.  A row
+ * 0); scores are scale * q.k, with softcap > 0 (at most 512) softcap * tanh(score / softcap).
+ * q and out are [rows, Hq, D] fp16, the sequences' tokens one after the other; statistics are
+ * fp32.  A row
  * whose scores are all -Inf gets zeros; NaN and Inf in K or V reach the rows that see their key
  * (an e4m3 code of NaN, which no call here writes, may reach any row of its sequence).  q and
  * out may be one buffer.

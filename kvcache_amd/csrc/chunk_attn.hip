@@ -359,6 +359,8 @@ int kvc_paged_chunk_attn(const void* q, void* out, const void* k_pool, const voi
             return set_error(KVC_ERR_ARG, "rows and the plan's counts must be >= 0");
         if (!std::isfinite(scale)) return set_error(KVC_ERR_ARG, "scale must be finite");
         if (!(softcap >= 0.f) || !std::isfinite(softcap)) return set_error(KVC_ERR_ARG, "softcap must be >= 0 and finite");
+        // (cap - 2 cap / (1 + e^(2x / cap)) is off by cap 2^-23: at 512 a probability by 2^-14)
+        if (softcap > 512.f) return set_error(KVC_ERR_UNSUPPORTED, "softcap must be at most 512 (0: none)");
         if (rows == 0 || n_units <= 1) return KVC_OK;
         if ((long long)n_units * Hkv > INT_MAX) return set_error(KVC_ERR_UNSUPPORTED, "at most 2^31 - 1 workgroups");
         if (!q || !out || !k_pool || !v_pool || !table_all || table_len <= 0 || !work)

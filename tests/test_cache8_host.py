@@ -85,6 +85,7 @@ def test_chunk_attention_unsupported_and_workspace():
     refused(N.KVC_ERR_UNSUPPORTED, attn, D=80)
     refused(N.KVC_ERR_UNSUPPORTED, attn, kv_dtype=N.KVC_F32)
     refused(N.KVC_ERR_UNSUPPORTED, attn, n_units=1 << 30, Hkv=8)
+    refused(N.KVC_ERR_UNSUPPORTED, attn, softcap=513.0)
     need = ops.chunk_workspace_size(8, 2, 64, (100, 50))
     assert need >= 2 * 100 * (64 + 2) * 4 + 2 * 50 * 2 * 64 * 2 and ops.chunk_workspace_size(8, 2, 64, (0, 0)) == 0
     refused(N.KVC_ERR_WORKSPACE, attn, ws_rows=(100, 50), workspace=(P, need - 1))

@@ -133,7 +133,7 @@ def test_window(window, kv):
 
 
 @pytest.mark.parametrize("kv", ALL, ids=NAME.get)
-@pytest.mark.parametrize("cap,std", [(30.0, 1.0), (5.0, 6.0), (50.0, 30.0)])
+@pytest.mark.parametrize("cap,std", [(30.0, 1.0), (5.0, 6.0), (50.0, 30.0), (512.0, 1.0), (0.05, 1.0)])
 def test_softcap(cap, std, kv):
     Batch([70, 1, 3], [200, 333, 64], 14, 2, 64, 16, kv, k_std=std).check(cap=cap)
     Batch([5, 20], [40, 21], 4, 4, 32, 16, kv, k_std=std).check(cap=cap, scale=-0.2)
